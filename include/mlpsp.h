@@ -326,6 +326,40 @@ int mlpsp_group_rows(const int32_t* primitive_ids, int64_t num_records, int32_t 
                      const int32_t* relu_masks, int64_t* offsets, int64_t* order, float* x6_out, float* grad4_out,
                      int32_t* masks_out, void* scratch, int64_t scratch_bytes, void* stream);
 
+/* ---- rows of pixels to their primitives and back ---- */
+
+/* The place of every record among the records grouped by primitive (stable: records of one primitive keep their order):
+ * offsets[n+1] int64 as mlpsp_group_records writes them, slots[R] int32 with 0 <= slots[r] < R, a permutation.  An id outside
+ * [0, n) drops its record: it takes a place at offsets[n] or behind.  R < 2^31; scratch as mlpsp_group_records. */
+int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_records, int32_t n, int64_t* offsets, int32_t* slots,
+                        void* scratch, int64_t scratch_bytes, void* stream);
+
+/* *findings_host (HOST) receives MLPSP_ROUTE_BAD_OFFSETS when pixel_offsets[pixels+1] does not start at zero, end at records
+ * or ascend, else 0; the call waits for the answer. */
+#define MLPSP_ROUTE_BAD_OFFSETS 1
+int mlpsp_check_pixel_offsets(const int64_t* pixel_offsets, int64_t pixels, int64_t records, int32_t* findings_host, void* stream);
+
+/* In the three calls below the records of pixel p are fan * p .. fan * (p + 1) - 1 (pixel_offsets NULL, records = pixels * fan)
+ * or pixel_offsets[p] .. pixel_offsets[p + 1] - 1 (int64 [pixels + 1], from zero to records, ascending); slots and kept =
+ * offsets + n (DEVICE pointer) are those of mlpsp_route_records.  dtype: MLPSP_PRECISION_F32 / _F16 / _BF16, the element type of
+ * the rows; dim <= MLPSP_ROUTE_MAX_DIM.  Sums are taken in FP32 in the order of a pixel's records and rounded once; no atomics.
+ * Offsets or slots that break these rules are never followed out of the arrays; the rows they reach are undefined. */
+#define MLPSP_ROUTE_MAX_DIM 65536
+/* out[slots[r], :] = x[pixel(r), :]; the rows of dropped records are zero.  x [pixels, dim], out [records, dim]. */
+int mlpsp_dispatch_rows(const void* x, int32_t dtype, int64_t dim, int64_t pixels, int32_t fan, const int64_t* pixel_offsets,
+                        const int32_t* slots, int64_t records, const int64_t* kept, void* out, void* stream);
+/* out[p, :] = sum of weights[r] * y[slots[r], :] over the records r of p that are not dropped (rows of dropped records are not
+ * read); weights FP32 [records], or NULL for ones, which makes the call the gradient of mlpsp_dispatch_rows.  y [records, dim],
+ * out [pixels, dim]; a pixel without records gets zeros. */
+int mlpsp_combine_rows(const void* y, int32_t dtype, int64_t dim, const float* weights, int64_t pixels, int32_t fan,
+                       const int64_t* pixel_offsets, const int32_t* slots, int64_t records, const int64_t* kept, void* out,
+                       void* stream);
+/* grad_y[slots[r], :] = weights[r] * grad_out[p, :] (zero rows for dropped records) and grad_weights[r] = <grad_out[p, :],
+ * y[slots[r], :]> (zero for them); either output may be NULL, y too when there is no grad_weights. */
+int mlpsp_combine_rows_gradients(const void* grad_out, const void* y, int32_t dtype, int64_t dim, const float* weights,
+                                 int64_t pixels, int32_t fan, const int64_t* pixel_offsets, const int32_t* slots,
+                                 int64_t records, const int64_t* kept, void* grad_y, float* grad_weights, void* stream);
+
 /* prepare_groups (primitive_gemm.py:186-203): split every primitive's records into segments of at
  * most segment_size.  group_offsets[n+1] int64 is always written; of primitives/starts ([G] int64, may be
  * NULL) the first min(G, max_groups) entries are written, so a caller may ask for G first (max_groups = 0)

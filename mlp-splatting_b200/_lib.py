@@ -21,6 +21,7 @@ BIT_TILE_ORIGINS, BIT_CONE_TOO_WIDE, BIT_FEAT_INEXACT = 256, 512, 1024
 BIT_PIXEL_HITS = 32
 ORDER_PER_PIXEL = 2
 REVERSE_BAD_OFFSETS, REVERSE_BAD_IDS = 1, 2
+ROUTE_BAD_OFFSETS, ROUTE_MAX_DIM = 1, 65536
 PRECISION_F32, PRECISION_F16, PRECISION_BF16 = 0, 1, 2
 MAX_WAVES = 32
 GEOM_FLOATS = 16
@@ -112,6 +113,12 @@ _SIGS = {
     "mlpsp_group_records_scratch_bytes": (C.c_int64, [C.c_int64, C.c_int32]),
     "mlpsp_group_records": (C.c_int, [_fp, C.c_int64, C.c_int32, _fp, _fp, _fp, C.c_int64, _fp]),
     "mlpsp_group_rows": (C.c_int, [_fp, C.c_int64, C.c_int32, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, C.c_int64, _fp]),
+    "mlpsp_route_records": (C.c_int, [_fp, C.c_int64, C.c_int32, _fp, _fp, _fp, C.c_int64, _fp]),
+    "mlpsp_check_pixel_offsets": (C.c_int, [_fp, C.c_int64, C.c_int64, C.POINTER(C.c_int32), _fp]),
+    "mlpsp_dispatch_rows": (C.c_int, [_fp, C.c_int32, C.c_int64, C.c_int64, C.c_int32, _fp, _fp, C.c_int64, _fp, _fp, _fp]),
+    "mlpsp_combine_rows": (C.c_int, [_fp, C.c_int32, C.c_int64, _fp, C.c_int64, C.c_int32, _fp, _fp, C.c_int64, _fp, _fp, _fp]),
+    "mlpsp_combine_rows_gradients": (C.c_int, [_fp, _fp, C.c_int32, C.c_int64, _fp, C.c_int64, C.c_int32, _fp, _fp, C.c_int64, _fp,
+                                               _fp, _fp, _fp]),
     "mlpsp_prepare_groups": (C.c_int, [_fp, C.c_int32, C.c_int64, _fp, _fp, _fp, C.c_int64, C.POINTER(C.c_int64), _fp]),
     "mlpsp_prepare_groups_static": (C.c_int, [_fp, C.c_int32, C.c_int64, _fp, _fp, _fp, C.c_int64, C.POINTER(C.c_int64), _fp]),
 }

@@ -1,0 +1,334 @@
+// Rows of pixels on their way to the primitives that the pixels' records name, and back.
+//
+// The records of pixel p are fan * p .. fan * (p + 1) - 1, or pixel_offsets[p] .. pixel_offsets[p + 1] - 1; slots[r] is the place
+// of record r among the records grouped by primitive (mlpsp_route_records), *kept how many of these places belong to a
+// primitive; a record at *kept or behind is dropped.
+//   dispatch            out[slots[r], :] = x[pixel(r), :], rows of dropped records zero
+//   combine             out[p, :]        = sum over the records r of p of w[r] y[slots[r], :]
+//   combine gradients   dy[slots[r], :]  = w[r] dout[p, :],   dw[r] = <dout[p, :], y[slots[r], :]>
+// The gradient of dispatch is combine with weights of one.  Every kernel is pixel-major: a pixel's own row is read (or written)
+// once and the rows of its records are visited in their order, so a sum over records is taken in one order whatever the
+// launch looks like, in FP32, and rounded once; no atomics.  Bound: memory, one visit of every record's row.
+//
+// Rows move in pieces of up to 16 bytes (the widest that the row length and all addresses are a multiple of).  dispatch and combine
+// give a thread one piece of one pixel: neighbouring threads take neighbouring pieces, so the lines of a row are whole whatever its
+// length, and a short row does not idle lanes.
+#include "frame.cuh"
+#include <cuda_bf16.h>
+
+namespace mlpsp {
+
+constexpr int kRtThreads = 256;
+
+// where the records of a pixel lie; offsets that descend or leave the records are cut to them
+struct RouteView {
+  const int64_t* __restrict__ pixel_offsets;
+  const int32_t* __restrict__ slots;
+  const int64_t* __restrict__ kept;
+  int64_t pixels, records;
+  int32_t fan;
+};
+__device__ __forceinline__ void rt_range(const RouteView& v, int64_t p, int64_t& b, int64_t& e) {
+  if (v.pixel_offsets) {
+    b = min(max(__ldg(v.pixel_offsets + p), (int64_t)0), v.records);
+    e = min(max(__ldg(v.pixel_offsets + p + 1), b), v.records);
+  } else {
+    b = p * v.fan;
+    e = b + v.fan;
+  }
+}
+__device__ __forceinline__ uint32_t rt_kept(const RouteView& v) { return (uint32_t)min(max(__ldg(v.kept), (int64_t)0), v.records); }
+
+template <int B> struct RtPiece;
+template <> struct RtPiece<16> { using type = uint4; };
+template <> struct RtPiece<8> { using type = uint2; };
+template <> struct RtPiece<4> { using type = uint32_t; };
+template <> struct RtPiece<2> { using type = uint16_t; };
+
+__device__ __forceinline__ float rt_float(float x) { return x; }
+__device__ __forceinline__ float rt_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float rt_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T rt_round(float x);
+template <> __device__ __forceinline__ float rt_round<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half rt_round<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 rt_round<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// the pixel and the piece of this thread: `ppb` pixels of `cb` pieces each per block, blocks of pieces along y
+__device__ __forceinline__ bool rt_place(int pieces, int cb, int ppb, int64_t pixels, int64_t& p, int& c) {
+  const int local = threadIdx.x / cb;
+  p = (int64_t)blockIdx.x * ppb + local;
+  c = blockIdx.y * cb + (threadIdx.x - local * cb);
+  return local < ppb && p < pixels && c < pieces;
+}
+
+template <int B>
+__global__ void __launch_bounds__(kRtThreads) k_dispatch(const typename RtPiece<B>::type* __restrict__ x, RouteView v, int pieces,
+                                                         int cb, int ppb, typename RtPiece<B>::type* __restrict__ out) {
+  chain_wait();
+  chain_release();
+  using V = typename RtPiece<B>::type;
+  int64_t p, b, e;
+  int c;
+  if (!rt_place(pieces, cb, ppb, v.pixels, p, c)) return;
+  rt_range(v, p, b, e);
+  if (b >= e) return;
+  const uint32_t kept = rt_kept(v), all = (uint32_t)v.records;
+  const V row = __ldg(x + (size_t)p * pieces + c);
+  const V zero = {};
+  for (int64_t r = b; r < e; r += 4) {
+    uint32_t s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s[u] = r + u < e ? (uint32_t)__ldg(v.slots + r + u) : all;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s[u] < all) out[(size_t)s[u] * pieces + c] = s[u] < kept ? row : zero;
+  }
+}
+
+template <typename T, int B>
+__global__ void __launch_bounds__(kRtThreads) k_combine(const typename RtPiece<B>::type* __restrict__ y, const float* __restrict__ weights,
+                                                        RouteView v, int pieces, int cb, int ppb,
+                                                        typename RtPiece<B>::type* __restrict__ out) {
+  chain_wait();
+  chain_release();
+  using V = typename RtPiece<B>::type;
+  constexpr int E = B / (int)sizeof(T);
+  int64_t p, b, e;
+  int c;
+  if (!rt_place(pieces, cb, ppb, v.pixels, p, c)) return;
+  rt_range(v, p, b, e);
+  const uint32_t kept = rt_kept(v);
+  float acc[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) acc[i] = 0.f;
+  for (int64_t r = b; r < e; r += 4) {
+    uint32_t s[4];
+    float w[4];
+    V row[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      s[u] = r + u < e ? (uint32_t)__ldg(v.slots + r + u) : 0xffffffffu;
+      w[u] = weights && r + u < e ? __ldg(weights + r + u) : 1.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s[u] < kept) row[u] = __ldg(y + (size_t)s[u] * pieces + c);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s[u] < kept) {
+        const T* f = reinterpret_cast<const T*>(&row[u]);
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[i] = fmaf(w[u], rt_float(f[i]), acc[i]);
+      }
+  }
+  V o;
+  T* f = reinterpret_cast<T*>(&o);
+#pragma unroll
+  for (int i = 0; i < E; ++i) f[i] = rt_round<T>(acc[i]);
+  out[(size_t)p * pieces + c] = o;
+}
+
+// `lanes` (a power of two) neighbouring threads take a pixel, so that <dout, y> is reduced by shuffles
+template <typename T, int B>
+__global__ void __launch_bounds__(kRtThreads) k_combine_grad(const typename RtPiece<B>::type* __restrict__ dout,
+                                                             const typename RtPiece<B>::type* __restrict__ y,
+                                                             const float* __restrict__ weights, RouteView v, int pieces, int lanes,
+                                                             typename RtPiece<B>::type* __restrict__ dy, float* __restrict__ dw) {
+  chain_wait();
+  chain_release();
+  using V = typename RtPiece<B>::type;
+  constexpr int E = B / (int)sizeof(T);
+  const int sub = threadIdx.x & (lanes - 1);
+  const int64_t p = ((int64_t)blockIdx.x * kRtThreads + threadIdx.x) / lanes;
+  int64_t b = 0, e = 0;
+  if (p < v.pixels) rt_range(v, p, b, e);
+  const uint32_t kept = rt_kept(v), all = (uint32_t)v.records;
+  const uint32_t group = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
+  for (int64_t r = b; r < e; ++r) {
+    const uint32_t s = (uint32_t)__ldg(v.slots + r);
+    const float w = weights ? __ldg(weights + r) : 1.f;
+    const bool live = s < kept;
+    float dot = 0.f;
+    for (int c = sub; c < pieces; c += lanes) {
+      const V g = __ldg(dout + (size_t)p * pieces + c);
+      const T* gf = reinterpret_cast<const T*>(&g);
+      if (dw && live) {
+        const V row = __ldg(y + (size_t)s * pieces + c);
+        const T* f = reinterpret_cast<const T*>(&row);
+#pragma unroll
+        for (int i = 0; i < E; ++i) dot = fmaf(rt_float(gf[i]), rt_float(f[i]), dot);
+      }
+      if (dy && s < all) {
+        V o = {};
+        T* of = reinterpret_cast<T*>(&o);
+        if (live)
+#pragma unroll
+          for (int i = 0; i < E; ++i) of[i] = rt_round<T>(w * rt_float(gf[i]));
+        dy[(size_t)s * pieces + c] = o;
+      }
+    }
+    if (dw) {
+      for (int o = lanes >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(group, dot, o);
+      if (sub == 0) dw[r] = dot;
+    }
+  }
+}
+
+// bit 0: the pixel offsets do not start at zero, end at the record count or ascend
+__global__ void k_route_check(const int64_t* __restrict__ offsets, int64_t pixels, int64_t records, volatile int32_t* __restrict__ found) {
+  chain_wait();
+  chain_release();
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+  bool bad = false;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i <= pixels; i += stride) {
+    const int64_t o = __ldg(offsets + i);
+    bad |= i == 0 ? o != 0 : o < __ldg(offsets + i - 1);
+    bad |= i == pixels && o != records;
+  }
+  if (bad) *found = MLPSP_ROUTE_BAD_OFFSETS;
+}
+
+// the widest piece that divides the row and all addresses
+static int rt_piece(int64_t row_bytes, std::initializer_list<const void*> ptrs) {
+  uintptr_t all = (uintptr_t)row_bytes;
+  for (const void* q : ptrs) all |= reinterpret_cast<uintptr_t>(q);
+  return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+}
+
+static int rt_check(const char* who, const RouteView& v, int64_t dim, int32_t dtype) {
+  MLPSP_REQUIRE(dtype == MLPSP_PRECISION_F32 || dtype == MLPSP_PRECISION_F16 || dtype == MLPSP_PRECISION_BF16, MLPSP_E_ARG,
+                "%s: unknown element type %d", who, dtype);
+  MLPSP_REQUIRE(v.pixels >= 0 && v.records >= 0 && v.fan >= 0 && dim >= 1, MLPSP_E_ARG, "%s: bad sizes", who);
+  MLPSP_REQUIRE(v.pixels < (1ll << 31) && v.records < (1ll << 31) && dim <= MLPSP_ROUTE_MAX_DIM, MLPSP_E_LIMIT,
+                "%s: more than 2^31-1 pixels or records, or rows longer than %d", who, MLPSP_ROUTE_MAX_DIM);
+  MLPSP_REQUIRE(v.pixel_offsets || v.pixels * v.fan == v.records, MLPSP_E_ARG, "%s: the record count is not pixels x fan", who);
+  MLPSP_REQUIRE(v.kept && (v.records == 0 || v.slots), MLPSP_E_ARG, "%s: null pointer", who);
+  return MLPSP_OK;
+}
+
+struct RtShape { int pieces, cb, ppb; dim3 grid, block; };
+static RtShape rt_shape(int64_t row_bytes, int piece, int64_t pixels) {
+  RtShape s;
+  s.pieces = (int)(row_bytes / piece);
+  s.cb = std::min(s.pieces, kRtThreads);
+  s.ppb = kRtThreads / s.cb;
+  s.grid = dim3((unsigned)((pixels + s.ppb - 1) / s.ppb), (unsigned)((s.pieces + s.cb - 1) / s.cb));
+  s.block = dim3((unsigned)((s.ppb * s.cb + 31) / 32 * 32));
+  return s;
+}
+
+template <int B>
+static void dispatch_rows(const void* x, const RouteView& v, int64_t row_bytes, void* out, cudaStream_t st) {
+  using V = typename RtPiece<B>::type;
+  const RtShape s = rt_shape(row_bytes, B, v.pixels);
+  launch_chained(k_dispatch<B>, s.grid, s.block, 0, st, static_cast<const V*>(x), v, s.pieces, s.cb, s.ppb, static_cast<V*>(out));
+}
+
+template <typename T, int B>
+static void combine_rows(const void* y, const float* weights, const RouteView& v, int64_t row_bytes, void* out, cudaStream_t st) {
+  using V = typename RtPiece<B>::type;
+  const RtShape s = rt_shape(row_bytes, B, v.pixels);
+  launch_chained(k_combine<T, B>, s.grid, s.block, 0, st, static_cast<const V*>(y), weights, v, s.pieces, s.cb, s.ppb, static_cast<V*>(out));
+}
+
+template <typename T, int B>
+static void combine_grad(const void* dout, const void* y, const float* weights, const RouteView& v, int64_t row_bytes, void* dy,
+                         float* dw, cudaStream_t st) {
+  using V = typename RtPiece<B>::type;
+  const int pieces = (int)(row_bytes / B);
+  int lanes = 1;
+  while (lanes < 32 && lanes < pieces) lanes *= 2;
+  const int64_t per_block = kRtThreads / lanes;
+  launch_chained(k_combine_grad<T, B>, dim3((unsigned)((v.pixels + per_block - 1) / per_block)), dim3(kRtThreads), 0, st,
+                 static_cast<const V*>(dout), static_cast<const V*>(y), weights, v, pieces, lanes, static_cast<V*>(dy), dw);
+}
+
+}  // namespace mlpsp
+
+using namespace mlpsp;
+
+#define MLPSP_BY_PIECE(T, call)             \
+  switch (piece) {                          \
+    case 16: call(T, 16); break;            \
+    case 8: call(T, 8); break;              \
+    case 4: call(T, 4); break;              \
+    default: call(T, 2); break;             \
+  }
+#define MLPSP_BY_TYPE(call)                                                                                       \
+  if (dtype == MLPSP_PRECISION_F32) {                                                                             \
+    if (piece == 16) call(float, 16); else if (piece == 8) call(float, 8); else call(float, 4);                   \
+  } else if (dtype == MLPSP_PRECISION_F16) { MLPSP_BY_PIECE(__half, call) } else { MLPSP_BY_PIECE(__nv_bfloat16, call) }
+
+extern "C" int mlpsp_check_pixel_offsets(const int64_t* pixel_offsets, int64_t pixels, int64_t records, int32_t* findings_host,
+                                         void* stream) {
+  MLPSP_REQUIRE(pixel_offsets && findings_host && pixels >= 0 && records >= 0, MLPSP_E_ARG, "mlpsp_check_pixel_offsets: bad arguments");
+  cudaStream_t st = (cudaStream_t)stream;
+  HostWords& hw = host_words();
+  cudaEvent_t ev = nullptr;
+  const int rc = hw.open(&ev);
+  if (rc) return rc;
+  hw.word[0] = 0;
+  LaunchScope scope(kKMisc, 1, st);
+  launch_chained(k_route_check, dim3((unsigned)std::min<int64_t>(sm_count() * 8, pixels / 1024 + 1)), dim3(256), 0, st, pixel_offsets, pixels,
+                 records, static_cast<volatile int32_t*>(hw.word));
+  MLPSP_CUDA_OK(cudaGetLastError());
+  MLPSP_CUDA_OK(cudaEventRecord(ev, st));
+  MLPSP_CUDA_OK(cudaEventSynchronize(ev));
+  *findings_host = *static_cast<volatile int32_t*>(hw.word);
+  return MLPSP_OK;
+}
+
+extern "C" int mlpsp_dispatch_rows(const void* x, int32_t dtype, int64_t dim, int64_t pixels, int32_t fan, const int64_t* pixel_offsets,
+                                   const int32_t* slots, int64_t records, const int64_t* kept, void* out, void* stream) {
+  const RouteView v{pixel_offsets, slots, kept, pixels, records, fan};
+  const int rc = rt_check("mlpsp_dispatch_rows", v, dim, dtype);
+  if (rc) return rc;
+  if (pixels == 0 || records == 0) return MLPSP_OK;
+  MLPSP_REQUIRE(x && out, MLPSP_E_ARG, "mlpsp_dispatch_rows: null pointer");
+  cudaStream_t st = (cudaStream_t)stream;
+  const int64_t row = dim * (dtype == MLPSP_PRECISION_F32 ? 4 : 2);
+  LaunchScope scope(kKMisc, 1, st);
+  switch (rt_piece(row, {x, out})) {
+    case 16: dispatch_rows<16>(x, v, row, out, st); break;
+    case 8: dispatch_rows<8>(x, v, row, out, st); break;
+    case 4: dispatch_rows<4>(x, v, row, out, st); break;
+    default: dispatch_rows<2>(x, v, row, out, st); break;
+  }
+  return cuda_check(cudaGetLastError(), "dispatch_rows");
+}
+
+extern "C" int mlpsp_combine_rows(const void* y, int32_t dtype, int64_t dim, const float* weights, int64_t pixels, int32_t fan,
+                                  const int64_t* pixel_offsets, const int32_t* slots, int64_t records, const int64_t* kept, void* out,
+                                  void* stream) {
+  const RouteView v{pixel_offsets, slots, kept, pixels, records, fan};
+  const int rc = rt_check("mlpsp_combine_rows", v, dim, dtype);
+  if (rc) return rc;
+  if (pixels == 0) return MLPSP_OK;
+  MLPSP_REQUIRE(out && (y || records == 0), MLPSP_E_ARG, "mlpsp_combine_rows: null pointer");
+  cudaStream_t st = (cudaStream_t)stream;
+  const int64_t row = dim * (dtype == MLPSP_PRECISION_F32 ? 4 : 2);
+  const int piece = rt_piece(row, {y, out});
+  LaunchScope scope(kKMisc, 1, st);
+#define MLPSP_CALL(T, B) combine_rows<T, B>(y, weights, v, row, out, st)
+  MLPSP_BY_TYPE(MLPSP_CALL)
+#undef MLPSP_CALL
+  return cuda_check(cudaGetLastError(), "combine_rows");
+}
+
+extern "C" int mlpsp_combine_rows_gradients(const void* grad_out, const void* y, int32_t dtype, int64_t dim, const float* weights,
+                                            int64_t pixels, int32_t fan, const int64_t* pixel_offsets, const int32_t* slots,
+                                            int64_t records, const int64_t* kept, void* grad_y, float* grad_weights, void* stream) {
+  const RouteView v{pixel_offsets, slots, kept, pixels, records, fan};
+  const int rc = rt_check("mlpsp_combine_rows_gradients", v, dim, dtype);
+  if (rc) return rc;
+  if (pixels == 0 || records == 0) return MLPSP_OK;
+  MLPSP_REQUIRE(grad_out && (grad_y || grad_weights) && (y || !grad_weights), MLPSP_E_ARG, "mlpsp_combine_rows_gradients: null pointer");
+  cudaStream_t st = (cudaStream_t)stream;
+  const int64_t row = dim * (dtype == MLPSP_PRECISION_F32 ? 4 : 2);
+  const int piece = rt_piece(row, {grad_out, y, grad_y});
+  LaunchScope scope(kKMisc, 1, st);
+#define MLPSP_CALL(T, B) combine_grad<T, B>(grad_out, y, weights, v, row, grad_y, grad_weights, st)
+  MLPSP_BY_TYPE(MLPSP_CALL)
+#undef MLPSP_CALL
+  return cuda_check(cudaGetLastError(), "combine_rows_gradients");
+}

@@ -102,3 +102,216 @@ def primitive_records_reverse(ids, offsets, x6, raw, log_scales, quats, grad_rgb
     if found.value & L.REVERSE_BAD_IDS:
         raise ValueError("record primitive ids out of range")
     return [d4, gp, gs, gq]
+
+
+# ---- rows of pixels to the primitives that their records name, and back ----
+_ROW_TYPES = {torch.float32: L.PRECISION_F32, torch.float16: L.PRECISION_F16, torch.bfloat16: L.PRECISION_BF16}
+
+
+@dataclass(frozen=True)
+class RecordRoute:
+    """Where the records of `pixels` pixels lie once they are grouped by primitive.
+
+    offsets      int64 [N+1]: the records of primitive i take the places offsets[i] .. offsets[i+1]-1, as in a PrimitiveCSR
+    slots        int32 [R], a permutation: the place of every record; places at offsets[N] and behind are those of dropped
+                 records (primitive id outside [0, N))
+    fan          records per pixel, or 0 with pixel_offsets int64 [pixels+1]: first record of every pixel, then R
+    Kernels never follow slots or offsets out of the tensors they index."""
+
+    offsets: torch.Tensor
+    slots: torch.Tensor
+    pixels: int
+    fan: int
+    pixel_offsets: torch.Tensor | None = None
+
+    @property
+    def records(self):
+        return int(self.slots.numel())
+
+
+def _check_route(route, *tensors):
+    if not isinstance(route, RecordRoute):
+        raise TypeError("route must be a RecordRoute, as route_records returns it")
+    slots, offsets, first = route.slots, route.offsets, route.pixel_offsets
+    for t in (slots, offsets, first, *tensors):
+        if t is not None and not (t.is_cuda and t.is_contiguous() and t.device == slots.device):
+            raise ValueError("all inputs must be contiguous tensors on one CUDA device")
+    if slots.dtype != torch.int32 or offsets.dtype != torch.int64 or offsets.numel() < 1:
+        raise ValueError("slots must be int32 and offsets int64 with the initial zero")
+    if first is None:
+        if route.pixels < 0 or route.fan < 0 or route.pixels * route.fan != slots.numel():
+            raise ValueError("the record count must be pixels x fan")
+    elif first.dtype != torch.int64 or first.ndim != 1 or first.numel() != route.pixels + 1:
+        raise ValueError("pixel offsets must be int64 with one entry more than pixels")
+
+
+def _check_rows(name, rows, count):
+    if rows.dtype not in _ROW_TYPES:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16")
+    if rows.ndim != 2 or rows.shape[0] != count or not 1 <= rows.shape[1] <= L.ROUTE_MAX_DIM:
+        raise ValueError(f"{name} must have shape ({count}, 1..{L.ROUTE_MAX_DIM}), got {tuple(rows.shape)}")
+
+
+def _check_weights(weights, route):
+    if weights is not None and (weights.dtype != torch.float32 or weights.numel() != route.records):
+        raise ValueError("weights must be float32, one for every record")
+
+
+def _route_args(route):
+    """(pixels, fan, pixel_offsets, slots, records, kept) of the C calls."""
+    return (route.pixels, 0 if route.pixel_offsets is not None else route.fan, L.ptr(route.pixel_offsets), L.ptr(route.slots),
+            route.records, route.offsets.data_ptr() + 8 * (route.offsets.numel() - 1))
+
+
+@torch.no_grad()
+def route_records(primitive_ids: torch.Tensor, num_primitives: int, pixel_offsets: torch.Tensor | None = None, *,
+                  check: bool = True) -> RecordRoute:
+    """The places of a frame's records among the records grouped by primitive (a stable grouping, as group_records).
+
+    primitive_ids: int32 or int64 [pixels, fan], fan primitives for every pixel, or [R] with pixel_offsets int64
+    [pixels+1] (the lists of render_tiles_training_records).  An id outside [0, num_primitives), -1 by convention, drops its
+    record.  With pixel_offsets the call waits for their check (ValueError) unless check is False."""
+    first = pixel_offsets
+    if not primitive_ids.is_cuda:
+        raise RuntimeError("route_records runs on a CUDA device; there is no CPU path")
+    if primitive_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError("primitive ids must be int32 or int64")
+    if first is None:
+        if primitive_ids.ndim != 2:
+            raise ValueError("primitive_ids must be [pixels, fan], or [records] with pixel_offsets")
+        pixels, fan = (int(d) for d in primitive_ids.shape)
+    else:
+        if primitive_ids.ndim != 1:
+            raise ValueError("primitive_ids must be [records] when pixel_offsets is given")
+        if first.ndim != 1 or first.dtype != torch.int64 or first.numel() < 1 or not first.is_contiguous() \
+                or first.device != primitive_ids.device:
+            raise ValueError("pixel offsets must be contiguous int64 with the initial zero, on the ids' device")
+        pixels, fan = int(first.numel()) - 1, 0
+    n, R = int(num_primitives), int(primitive_ids.numel())
+    if not 0 <= n < 2 ** 31 - 1 or pixels >= 2 ** 31 or R >= 2 ** 31:
+        raise ValueError("primitives, pixels and records must be below 2^31")
+    if primitive_ids.dtype == torch.int64:      # ids beyond 32 bits are out of range, not wrapped into it
+        primitive_ids = primitive_ids.clamp(-1, n).to(torch.int32)
+    lib, dev = L.load(), primitive_ids.device
+    ids = primitive_ids.contiguous()
+    if first is not None and check and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("route_records waits for the check of pixel_offsets: pass check=False inside a graph capture")
+    offsets = torch.empty(n + 1, device=dev, dtype=torch.int64)
+    slots = torch.empty(R, device=dev, dtype=torch.int32)
+    nbytes = int(lib.mlpsp_group_records_scratch_bytes(R, n))
+    scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    found = C.c_int32(0)
+    with _on(dev):
+        st = _stream_ptr(dev)
+        if first is not None and check:
+            L.check(lib.mlpsp_check_pixel_offsets(L.ptr(first), pixels, R, C.byref(found), st), "mlpsp_check_pixel_offsets")
+            if found.value & L.ROUTE_BAD_OFFSETS:
+                raise ValueError("pixel offsets must start at zero, end at the record count and be monotone")
+        L.check(lib.mlpsp_route_records(L.ptr(ids), R, n, L.ptr(offsets), L.ptr(slots), L.ptr(scratch), nbytes, st),
+                "mlpsp_route_records")
+    return RecordRoute(offsets, slots, pixels, fan, first)
+
+
+def _dispatch(x, route):
+    _check_route(route, x)
+    _check_rows("x", x, route.pixels)
+    out = torch.empty((route.records, x.shape[1]), device=x.device, dtype=x.dtype)
+    with _on(x.device):
+        L.check(L.load().mlpsp_dispatch_rows(L.ptr(x), _ROW_TYPES[x.dtype], x.shape[1], *_route_args(route), L.ptr(out),
+                                             _stream_ptr(x.device)), "mlpsp_dispatch_rows")
+    return out
+
+
+def _combine(y, route, weights, name="y"):
+    _check_route(route, y, weights)
+    _check_rows(name, y, route.records)
+    _check_weights(weights, route)
+    out = torch.empty((route.pixels, y.shape[1]), device=y.device, dtype=y.dtype)
+    with _on(y.device):
+        L.check(L.load().mlpsp_combine_rows(L.ptr(y), _ROW_TYPES[y.dtype], y.shape[1], L.ptr(weights), *_route_args(route), L.ptr(out),
+                                            _stream_ptr(y.device)), "mlpsp_combine_rows")
+    return out
+
+
+def _combine_gradients(grad_out, y, route, weights, want_y, want_weights):
+    _check_route(route, grad_out, y, weights)
+    _check_rows("grad_out", grad_out, route.pixels)
+    _check_rows("y", y, route.records)
+    if y.dtype != grad_out.dtype or y.shape[1] != grad_out.shape[1]:
+        raise ValueError("grad_out and y must have one element type and row length")
+    _check_weights(weights, route)
+    grad_y = torch.empty_like(y) if want_y else None
+    grad_weights = torch.empty_like(weights) if want_weights else None
+    if want_y or want_weights:
+        with _on(y.device):
+            L.check(L.load().mlpsp_combine_rows_gradients(
+                L.ptr(grad_out), L.ptr(y), _ROW_TYPES[y.dtype], y.shape[1], L.ptr(weights), *_route_args(route), L.ptr(grad_y),
+                L.ptr(grad_weights), _stream_ptr(y.device)), "mlpsp_combine_rows_gradients")
+    return grad_y, grad_weights
+
+
+def _saved_route(ctx, offsets, slots, first):
+    return RecordRoute(offsets, slots, ctx.pixels, ctx.fan, first)
+
+
+class _DispatchRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, route):
+        ctx.save_for_backward(route.offsets, route.slots, route.pixel_offsets)
+        ctx.pixels, ctx.fan = route.pixels, route.fan
+        return _dispatch(x, route)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _combine(grad.contiguous(), _saved_route(ctx, *ctx.saved_tensors), None, "grad_rows"), None
+
+
+class _CombineRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, route, weights):
+        ctx.save_for_backward(y, weights, route.offsets, route.slots, route.pixel_offsets)
+        ctx.pixels, ctx.fan = route.pixels, route.fan
+        return _combine(y, route, weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        y, weights, *where = ctx.saved_tensors
+        grad_y, grad_weights = _combine_gradients(grad.contiguous(), y, _saved_route(ctx, *where), weights, ctx.needs_input_grad[0],
+                                                  weights is not None and ctx.needs_input_grad[2])
+        return grad_y, None, grad_weights
+
+
+def dispatch_rows(x: torch.Tensor, route: RecordRoute) -> torch.Tensor:
+    """Every pixel's row to its records, grouped by primitive: out[route.slots[r]] = x[pixel of r]; the rows of dropped
+    records, from route.offsets[N] on, are zero.  x [pixels, D] float32, float16 or bfloat16, contiguous; out [records, D].
+    Differentiable in x; dispatch_rows_gradient is the gradient without autograd."""
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _DispatchRows.apply(x, route)
+    return _dispatch(x, route)
+
+
+@torch.no_grad()
+def dispatch_rows_gradient(grad_rows: torch.Tensor, route: RecordRoute) -> torch.Tensor:
+    """Gradient of dispatch_rows with respect to x [pixels, D]: the sums of every pixel's records' rows of grad_rows [records, D],
+    in FP32 in the order of the records, rounded once; rows of dropped records are not read."""
+    return _combine(grad_rows, route, None, "grad_rows")
+
+
+def combine_rows(y: torch.Tensor, route: RecordRoute, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """The records' rows back to their pixels: out[p] = sum of weights[r] * y[route.slots[r]] over the records r of p (ones
+    without weights), in FP32 in the order of the records, rounded once to y's type.  y [records, D] grouped by primitive,
+    float32, float16 or bfloat16, contiguous; weights float32, one per record in record order ([pixels, fan] or [records]).  Rows
+    of dropped records are not read; a pixel without records gets zeros.  Differentiable in y and weights;
+    combine_rows_gradients gives both gradients without autograd."""
+    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
+        return _CombineRows.apply(y, route, weights)
+    return _combine(y, route, weights)
+
+
+@torch.no_grad()
+def combine_rows_gradients(grad_out: torch.Tensor, y: torch.Tensor, route: RecordRoute, weights: torch.Tensor | None = None):
+    """(gradient of combine_rows with respect to y [records, D], with respect to weights in their shape, or None without
+    weights) from grad_out [pixels, D].  Zero for dropped records."""
+    return _combine_gradients(grad_out, y, route, weights, True, weights is not None)

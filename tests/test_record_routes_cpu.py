@@ -1,0 +1,39 @@
+"""Argument errors of the row routes, found on the host."""
+import ctypes
+
+import pytest
+import torch
+
+from mlp_splatting_b200 import _lib as L
+from mlp_splatting_b200 import primitive_csr as pc
+
+FAKE = 0x1000      # never dereferenced: the calls stop at their argument checks
+
+
+def test_c_entries_check_their_arguments():
+    lib = L.load()
+    assert lib.mlpsp_dispatch_rows(FAKE, 5, 4, 2, 2, None, FAKE, 4, FAKE, FAKE, None) == -1
+    assert b"unknown element type 5" in lib.mlpsp_last_error()
+    assert lib.mlpsp_dispatch_rows(FAKE, 0, 0, 2, 2, None, FAKE, 4, FAKE, FAKE, None) == -1
+    assert lib.mlpsp_dispatch_rows(FAKE, 0, 65537, 2, 2, None, FAKE, 4, FAKE, FAKE, None) == -4
+    assert lib.mlpsp_dispatch_rows(FAKE, 0, 4, 2, 2, None, FAKE, 5, FAKE, FAKE, None) == -1
+    assert b"pixels x fan" in lib.mlpsp_last_error()
+    assert lib.mlpsp_combine_rows(FAKE, 0, 4, None, 1 << 31, 0, FAKE, FAKE, 4, FAKE, FAKE, None) == -4
+    assert lib.mlpsp_combine_rows(FAKE, 0, 4, None, 2, 2, None, None, 4, FAKE, FAKE, None) == -1
+    assert b"null pointer" in lib.mlpsp_last_error()
+    assert lib.mlpsp_combine_rows_gradients(FAKE, FAKE, 0, 4, None, 2, 2, None, FAKE, 4, FAKE, None, None, None) == -1
+    assert lib.mlpsp_combine_rows_gradients(FAKE, None, 0, 4, None, 2, 2, None, FAKE, 4, FAKE, FAKE, FAKE, None) == -1
+    assert lib.mlpsp_route_records(FAKE, 1 << 31, 4, FAKE, FAKE, FAKE, 1 << 40, None) == -4
+    assert lib.mlpsp_route_records(FAKE, 4, 4, FAKE, None, FAKE, 1 << 20, None) == -1
+    assert lib.mlpsp_route_records(FAKE, 4, 4, FAKE, FAKE, FAKE, 8, None) == -2
+    assert lib.mlpsp_check_pixel_offsets(None, 1, 1, ctypes.byref(ctypes.c_int32()), None) == -1
+    # nothing to do: no launch, no pointer is looked at
+    assert lib.mlpsp_dispatch_rows(None, 0, 4, 0, 2, None, None, 0, FAKE, None, None) == 0
+
+
+def test_there_is_no_cpu_path():
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        pc.route_records(torch.zeros(3, 2, dtype=torch.int32), 4)
+    route = pc.RecordRoute(torch.zeros(2, dtype=torch.int64), torch.zeros(4, dtype=torch.int32), 2, 2)
+    with pytest.raises(ValueError, match="one CUDA device"):
+        pc.dispatch_rows(torch.zeros(2, 3), route)

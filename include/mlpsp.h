@@ -443,6 +443,29 @@ int mlpsp_weight_gradients(const mlpsp_scene* scene, const int64_t* offsets, con
                            float loss_scale, float* dW1, float* db1, float* dW2, float* db2, float* dW3, float* db3,
                            void* scratch, int64_t scratch_bytes, int32_t* nonfinite_host, void* stream);
 
+/* ---- weight updates by orthogonalised momentum ---- */
+
+/* Newton-Schulz iteration of n matrices [rows, cols], contiguous and row-major: X = U / max(|U|_F, eps), then `steps` times
+ * X <- a X + (b A + c A^2) X with A = X X^T (on the shorter side), which takes the singular values of U towards one.
+ * dtype: MLPSP_PRECISION_F32 / _F16 / _BF16, the element type of update and out (the same array or one apart); the iteration has FP32
+ * accuracy whatever the type, and the result is rounded once.  A matrix of zeros gives zeros, one that holds an infinity or a NaN gives
+ * NaN, alone.  Coefficients under which singular values leave [0, 4] within the steps are refused, as are more than
+ * MLPSP_MUON_MAX_SMALL rows or columns on the shorter and MLPSP_MUON_MAX_LARGE on the longer side; 1e-15 <= eps <= 1, 1 <= steps <= 32.
+ * status (or NULL): MLPSP_ST_TIMEOUT when a device-side wait gave up, results then invalid; only shapes for which
+ * mlpsp_orthogonalize_waits answers 1 wait. */
+#define MLPSP_MUON_MAX_SMALL 128
+#define MLPSP_MUON_MAX_LARGE 2048
+int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols);
+int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a, double b,
+                        double c, double eps, void* out, int32_t* status, void* stream);
+/* One step, in place, on n weight matrices and their momenta (FP32): m <- m + (1 - momentum)(g - m), U = g + momentum (m - g)
+ * (nesterov) or m, w <- (1 - lr weight_decay) w - lr scale X(U), X as above.  grads [n, rows, cols] of grad_dtype.
+ * active [n] (bytes, or NULL): matrices whose byte is zero keep weights and momenta and are not read.  The four arrays may not
+ * overlap. */
+int mlpsp_muon_step(float* weights, const void* grads, int32_t grad_dtype, float* momenta, const uint8_t* active, int64_t n, int32_t rows,
+                    int32_t cols, double lr, double momentum, int32_t nesterov, double weight_decay, double scale, int32_t steps,
+                    double a, double b, double c, double eps, int32_t* status, void* stream);
+
 /* ---- the step after the feature map: feature decoder and text query ---- */
 
 /* The reference's FeatureUpsampleDecoder (scannet/feature_decoder.py:5-19): conv 1x1 -> ReLU -> conv 3x3 (zero

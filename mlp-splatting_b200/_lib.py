@@ -22,6 +22,7 @@ BIT_PIXEL_HITS = 32
 ORDER_PER_PIXEL = 2
 REVERSE_BAD_OFFSETS, REVERSE_BAD_IDS = 1, 2
 ROUTE_BAD_OFFSETS, ROUTE_MAX_DIM = 1, 65536
+MUON_MAX_SMALL, MUON_MAX_LARGE = 128, 2048
 PRECISION_F32, PRECISION_F16, PRECISION_BF16 = 0, 1, 2
 MAX_WAVES = 32
 GEOM_FLOATS = 16
@@ -86,6 +87,10 @@ _SIGS = {
     "mlpsp_weight_gradients_scratch_bytes": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32]),
     "mlpsp_weight_gradients": (C.c_int, [C.POINTER(Scene), _fp, _fp, _fp, _fp, C.c_int64, C.c_int32, C.c_int32, C.c_float,
                                          _fp, _fp, _fp, _fp, _fp, _fp, _fp, C.c_int64, _fp, _fp]),
+    "mlpsp_orthogonalize_waits": (C.c_int, [C.c_int32, C.c_int32]),
+    "mlpsp_orthogonalize": (C.c_int, [_fp, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32] + [C.c_double] * 4 + [_fp, _fp, _fp]),
+    "mlpsp_muon_step": (C.c_int, [_fp, _fp, C.c_int32, _fp, _fp, C.c_int64, C.c_int32, C.c_int32, C.c_double, C.c_double, C.c_int32,
+                                  C.c_double, C.c_double, C.c_int32] + [C.c_double] * 4 + [_fp, _fp]),
     "mlpsp_decoder_packed_bytes": (C.c_int64, [C.POINTER(Decoder), C.c_int32]),
     "mlpsp_pack_decoder": (C.c_int, [C.POINTER(Decoder), C.c_int32, _fp, _fp, _fp]),
     "mlpsp_decode_features": (C.c_int, [C.POINTER(Decoder), C.c_int32, _fp, _fp, C.c_int32, C.c_int32, _fp, _fp, _fp, _fp]),

@@ -193,10 +193,14 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
       if (warp == 0) {
         if (elect_one()) {
           const uint64_t dh = smem_desc(xh, kNtChunk, 128), dl = smem_desc(xl, kNtChunk, 128);
+          // the small products first: the tensor core rounds a sum towards zero with every MMA
           for (int s = 0; s < groups; ++s) {
             const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4);
             mma_f16(tmem, dh + o, dl + o, idesc_a, s > 0);
             mma_f16(tmem, dl + o, dh + o, idesc_a, 1u);
+          }
+          for (int s = 0; s < groups; ++s) {
+            const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4);
             mma_f16(tmem, dh + o, dh + o, idesc_a, 1u);
           }
           mma_commit(bar);
@@ -276,6 +280,9 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
             const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4);
             mma_f16(tmem + kNtRows, dh + o, dl + o, idesc_a, s > 0);
             mma_f16(tmem + kNtRows, dl + o, dh + o, idesc_a, 1u);
+          }
+          for (int s = 0; s < 8; ++s) {
+            const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4);
             mma_f16(tmem + kNtRows, dh + o, dh + o, idesc_a, 1u);
           }
           mma_commit(bar);
@@ -312,6 +319,9 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
             const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4), n = (uint64_t)(s * 256 >> 4);
             mma_f16(tmem, ph + o, dl + n, idesc_x, s > 0);
             mma_f16(tmem, pl + o, dh + n, idesc_x, 1u);
+          }
+          for (int s = 0; s < 8; ++s) {
+            const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4), n = (uint64_t)(s * 256 >> 4);
             mma_f16(tmem, ph + o, dh + n, idesc_x, 1u);
           }
           mma_commit(bar);
@@ -410,19 +420,23 @@ int launch_ns_cluster(const NsArgs& q, cudaStream_t st) {
   return cuda_check(cudaLaunchKernelEx(&cfg, k_ns_cluster, q, np, cluster, pack, tiles), "orthogonalize");
 }
 
-// Whether the iteration stays in the binary16 range of the scaled operands: from singular values in [0, 1], values within [0, 4] and
-// |b s^2 + c s^4| within 32 after every step, followed on a grid of 4,096 points (the polynomials are of degree five).
+// Whether the iteration stays in the binary16 range of the scaled operands: from singular values in [0, 1], values within [-4, 4] and
+// |b s^2 + c s^4| within 32 after every step.  Both polynomials take their extremes over [0, top] at the ends or where their
+// derivatives vanish, quadratics in s^2.
 static bool ns_bounded(double a, double b, double c, int steps) {
   double top = 1.0;
   for (int it = 0; it < steps; ++it) {
     double next = 0.0;
-    for (int i = 0; i <= 4096; ++i) {
-      const double s = top * i / 4096.0, s2 = s * s, p = b * s2 + c * s2 * s2;
-      const double y = (a + p) * s;
+    const double disc = 9.0 * b * b - 20.0 * a * c, root = disc > 0.0 ? std::sqrt(disc) : 0.0;
+    const double at[] = {top * top, c != 0.0 ? -b / (2.0 * c) : 0.0, c != 0.0 ? (-3.0 * b + root) / (10.0 * c) : b != 0.0 ? -a / (3.0 * b) : 0.0,
+                         c != 0.0 ? (-3.0 * b - root) / (10.0 * c) : 0.0};
+    for (double s2 : at) {
+      s2 = s2 > 0.0 && s2 < top * top ? s2 : top * top;
+      const double p = b * s2 + c * s2 * s2, y = (a + p) * std::sqrt(s2);
       if (!(p >= -32.0 && p <= 32.0 && y >= -4.0 && y <= 4.0)) return false;
-      next = std::max(next, y < 0 ? -y : y);
+      next = std::max(next, std::fabs(y));
     }
-    top = next * 1.001;
+    top = std::max(next, 1e-30) * 1.001;
   }
   return true;
 }

@@ -13,37 +13,43 @@
 namespace mlpsp {
 
 __device__ __forceinline__ void ns_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void ns_mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b0));
 }
 __device__ __forceinline__ uint32_t ns_transpose(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 
 // fragments of a [16 MB x 8 NB] matrix: f[mb][nb][h] = rows 16 mb + 8 h + g, columns 8 nb + 2 t and + 1
 template <int MB, int NB> struct NsFrag { uint32_t hi[MB][NB][2], lo[MB][NB][2]; };
 
-// d += rows 16 mb.. of x times (rows 8 n.. of x)^T
+// The blocks of x x^T on and below the diagonal: d[mb * (mb + 1) + n] = rows 16 mb.. times rows 8 n.., n <= 2 mb + 1.  All of them
+// advance together, since an MMA takes four times as long to answer as to issue; the small products come first, so that the tensor
+// core's rounding of a sum towards zero meets the large ones only.
 template <int MB, int NB>
-__device__ __forceinline__ void ns_gram_tile(const NsFrag<MB, NB>& x, int mb, int n, float (&d)[4]) {
-  const int nm = n >> 1, nh = n & 1;
+__device__ __forceinline__ void ns_gram(const NsFrag<MB, NB>& x, float (&d)[MB * (MB + 1)][4]) {
 #pragma unroll
-  for (int k = 0; k + 1 < NB; k += 2) {
-    ns_mma(d, x.hi[mb][k][0], x.hi[mb][k][1], x.hi[mb][k + 1][0], x.hi[mb][k + 1][1], x.lo[nm][k][nh], x.lo[nm][k + 1][nh]);
-    ns_mma(d, x.lo[mb][k][0], x.lo[mb][k][1], x.lo[mb][k + 1][0], x.lo[mb][k + 1][1], x.hi[nm][k][nh], x.hi[nm][k + 1][nh]);
-    ns_mma(d, x.hi[mb][k][0], x.hi[mb][k][1], x.hi[mb][k + 1][0], x.hi[mb][k + 1][1], x.hi[nm][k][nh], x.hi[nm][k + 1][nh]);
-  }
-  if (NB & 1) {
-    constexpr int k = NB - 1;
-    ns_mma8(d, x.hi[mb][k][0], x.hi[mb][k][1], x.lo[nm][k][nh]);
-    ns_mma8(d, x.lo[mb][k][0], x.lo[mb][k][1], x.hi[nm][k][nh]);
-    ns_mma8(d, x.hi[mb][k][0], x.hi[mb][k][1], x.hi[nm][k][nh]);
+  for (int i = 0; i < MB * (MB + 1); ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
+#pragma unroll
+  for (int part = 0; part < 3; ++part) {
+    const auto& l = part == 1 ? x.lo : x.hi;
+    const auto& r = part == 0 ? x.lo : x.hi;
+#pragma unroll
+    for (int k = 0; k < NB; k += 2)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int n = 0; n < 2 * mb + 2; ++n) {
+          float(&o)[4] = d[mb * (mb + 1) + n];
+          if (k + 1 < NB) ns_mma(o, l[mb][k][0], l[mb][k][1], l[mb][(k + 1) % NB][0], l[mb][(k + 1) % NB][1], r[n >> 1][k][n & 1], r[n >> 1][(k + 1) % NB][n & 1]);
+          else ns_mma8(o, l[mb][k][0], l[mb][k][1], r[n >> 1][k][n & 1]);
+        }
   }
 }
 // blocks above the diagonal from those below
@@ -229,68 +235,86 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
 #pragma unroll
       for (int h = 0; h < KH; ++h) by[h] = ns_step(q, k2[h]);
       NsFrag<MB, 2 * MB> A;
+      {
+        float d[MB * (MB + 1)][4];
+        ns_gram(X, d);
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
+        for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-        for (int n = 0; n < 2 * mb + 2; ++n) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          ns_gram_tile(X, mb, n, d);
+          for (int n = 0; n < 2 * mb + 2; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float v0 = d[2 * h] * by[h % KH].gram, v1 = d[2 * h + 1] * by[h % KH].gram;
-            if (MB == 1) {
-              if (!(same >> (h * 4 + n * 2) & 1u)) v0 = 0.f;
-              if (!(same >> (h * 4 + n * 2 + 1) & 1u)) v1 = 0.f;
+            for (int h = 0; h < 2; ++h) {
+              const float(&o)[4] = d[mb * (mb + 1) + n];
+              float v0 = o[2 * h] * by[h % KH].gram, v1 = o[2 * h + 1] * by[h % KH].gram;
+              if (MB == 1) {
+                if (!(same >> (h * 4 + n * 2) & 1u)) v0 = 0.f;
+                if (!(same >> (h * 4 + n * 2 + 1) & 1u)) v1 = 0.f;
+              }
+              ns_split(v0, v1, A.hi[mb][n][h], A.lo[mb][n][h]);
             }
-            ns_split(v0, v1, A.hi[mb][n][h], A.lo[mb][n][h]);
-          }
-        }
+      }
       ns_mirror<MB>(A);
       NsFrag<MB, 2 * MB> P;
+      {
+        float d[MB * (MB + 1)][4];
+        ns_gram(A, d);
+        const float c = q.c * kNsUnscale;
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
+        for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-        for (int n = 0; n < 2 * mb + 2; ++n) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          ns_gram_tile(A, mb, n, d);
+          for (int n = 0; n < 2 * mb + 2; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 a = ns_join(A.hi[mb][n][h], A.lo[mb][n][h]);
-            ns_split(fmaf(q.b, a.x, q.c * (d[2 * h] * kNsUnscale)), fmaf(q.b, a.y, q.c * (d[2 * h + 1] * kNsUnscale)), P.hi[mb][n][h],
-                     P.lo[mb][n][h]);
-          }
-        }
+            for (int h = 0; h < 2; ++h) {
+              const float(&o)[4] = d[mb * (mb + 1) + n];
+              const float2 a = ns_join(A.hi[mb][n][h], A.lo[mb][n][h]);
+              ns_split(fmaf(q.b, a.x, c * o[2 * h]), fmaf(q.b, a.y, c * o[2 * h + 1]), P.hi[mb][n][h], P.lo[mb][n][h]);
+            }
+      }
       ns_mirror<MB>(P);
       const bool last = it + 1 == q.steps;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        uint32_t bh[MB][2], bl[MB][2];
+      for (int c0 = 0; c0 < NB; c0 += CH) {
+        uint32_t bh[CH][MB][2], bl[CH][MB][2];
+        float d[CH][MB][4];
 #pragma unroll
-        for (int k = 0; k < MB; ++k)
+        for (int u = 0; u < CH; ++u)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) { bh[k][h] = ns_transpose(X.hi[k][nb][h]); bl[k][h] = ns_transpose(X.lo[k][nb][h]); }
+          for (int k = 0; k < MB; ++k)
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < MB; ++k) {
-            ns_mma(d, P.hi[mb][2 * k][0], P.hi[mb][2 * k][1], P.hi[mb][2 * k + 1][0], P.hi[mb][2 * k + 1][1], bl[k][0], bl[k][1]);
-            ns_mma(d, P.lo[mb][2 * k][0], P.lo[mb][2 * k][1], P.lo[mb][2 * k + 1][0], P.lo[mb][2 * k + 1][1], bh[k][0], bh[k][1]);
-            ns_mma(d, P.hi[mb][2 * k][0], P.hi[mb][2 * k][1], P.hi[mb][2 * k + 1][0], P.hi[mb][2 * k + 1][1], bh[k][0], bh[k][1]);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 v = ns_join(X.hi[mb][nb][h], X.lo[mb][nb][h]);
-            const NsStep& f1 = by[h % KH];
-            const float v0 = fmaf(f1.a, v.x, d[2 * h] * f1.unscale), v1 = fmaf(f1.a, v.y, d[2 * h + 1] * f1.unscale);
-            if (last) {          // the result keeps its FP32 bits in the two words of the pair
-              X.hi[mb][nb][h] = __float_as_uint(v0);
-              X.lo[mb][nb][h] = __float_as_uint(v1);
-            } else {
-              ns_split(v0, v1, X.hi[mb][nb][h], X.lo[mb][nb][h]);
+            for (int h = 0; h < 2; ++h) {
+              bh[u][k][h] = ns_transpose(X.hi[k][c0 + u][h]);
+              bl[u][k][h] = ns_transpose(X.lo[k][c0 + u][h]);
+              d[u][k][2 * h] = d[u][k][2 * h + 1] = 0.f;
             }
-          }
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+          const auto& l = part == 1 ? P.lo : P.hi;
+          const auto& r = part == 0 ? bl : bh;
+#pragma unroll
+          for (int k = 0; k < MB; ++k)
+#pragma unroll
+            for (int u = 0; u < CH; ++u)
+#pragma unroll
+              for (int mb = 0; mb < MB; ++mb)
+                ns_mma(d[u][mb], l[mb][2 * k][0], l[mb][2 * k][1], l[mb][2 * k + 1][0], l[mb][2 * k + 1][1], r[u][k][0], r[u][k][1]);
         }
+#pragma unroll
+        for (int u = 0; u < CH; ++u)
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t &xh = X.hi[mb][c0 + u][h], &xl = X.lo[mb][c0 + u][h];
+              const float2 v = ns_join(xh, xl);
+              const NsStep& f1 = by[h % KH];
+              const float v0 = fmaf(f1.a, v.x, d[u][mb][2 * h] * f1.unscale), v1 = fmaf(f1.a, v.y, d[u][mb][2 * h + 1] * f1.unscale);
+              if (last) {          // the result keeps its FP32 bits in the two words of the pair
+                xh = __float_as_uint(v0);
+                xl = __float_as_uint(v1);
+              } else {
+                ns_split(v0, v1, xh, xl);
+              }
+            }
       }
     }
     const float nan = __int_as_float(0x7fffffff);

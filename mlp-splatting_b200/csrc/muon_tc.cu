@@ -8,7 +8,6 @@
 //
 // Every wait on an mbarrier is bounded; one that gives up raises MLPSP_ST_TIMEOUT and this CTA's slice of the result is not written.
 #include <cmath>
-#include <type_traits>
 #include "muon.cuh"
 
 namespace mlpsp {
@@ -55,6 +54,10 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
   char* const pah = pxl + np * (kNtChunk / 8);
   char* const pal = pah + 16 * kNtChunk;
   float4* const s_part = reinterpret_cast<float4*>(pal + 16 * kNtChunk);      // [2][128] squares of a row's halves: plain, shrunk, grown
+  // between the norms: [128] the diagonal of bA + cA^2, and [2][128] each the halves' sums of squares of a row of X and of A
+  float* const s_diag = reinterpret_cast<float*>(s_part);
+  float* const s_xsq = s_diag + kNtRows;
+  float* const s_asq = s_xsq + 2 * kNtRows;
   float4* const s_rank = s_part + 2 * kNtRows;                               // this CTA's sums, read by the cluster's others
   uint32_t* const s_word = reinterpret_cast<uint32_t*>(s_rank + 1);           // mbarrier (two words) | tensor memory | gave up
   const uint32_t bar = smem_u32(s_word);
@@ -118,8 +121,6 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
       }
       return v;
     };
-    using One = std::integral_constant<int, 1>;
-    using Four = std::integral_constant<int, 4>;
     for (int gr = half; gr < groups; gr += 2) {
       const int c = col0 + gr * 16;
       if (!in) break;
@@ -127,13 +128,13 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
           if (c + e < q.large) {
-            const NsVec<4> v = fetch(base + c + e, Four{}, true);
+            const NsVec<4> v = fetch(base + c + e, NsTag<4>{}, true);
 #pragma unroll
             for (int i = 0; i < 4; ++i) square(v.v[i]);
           }
       } else {
         for (int e = 0; e < 16; ++e)
-          if (c + e < q.large) square(fetch(base + (int64_t)(c + e) * q.cs, One{}, true).v[0]);
+          if (c + e < q.large) square(fetch(base + (int64_t)(c + e) * q.cs, NsTag<1>{}, true).v[0]);
       }
     }
     s_part[half * kNtRows + row] = ss;
@@ -157,6 +158,8 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
     const bool lost = start.lost;
     int k2 = start.k;
     // ---- pass two: X0 as binary16 pairs
+    __syncthreads();         // the norms' sums have been read
+    float xsq = 0.f;
     for (int gr = half; gr < groups; gr += 2) {
       const int c = col0 + gr * 16;
       float u[16];
@@ -167,17 +170,19 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
 #pragma unroll
           for (int e = 0; e < 16; e += 4)
             if (c + e < q.large) {
-              const NsVec<4> v = fetch(base + c + e, Four{}, false);
+              const NsVec<4> v = fetch(base + c + e, NsTag<4>{}, false);
 #pragma unroll
               for (int i = 0; i < 4; ++i) u[e + i] = v.v[i] * start.pre * start.inv;
             }
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (c + e < q.large) u[e] = fetch(base + (int64_t)(c + e) * q.cs, One{}, false).v[0] * start.pre * start.inv;
+            if (c + e < q.large) u[e] = fetch(base + (int64_t)(c + e) * q.cs, NsTag<1>{}, false).v[0] * start.pre * start.inv;
         }
       }
       uint32_t h[8], l[8];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) xsq = fmaf(u[e], u[e], xsq);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ns_split(u[2 * e], u[2 * e + 1], h[e], l[e]);
 #pragma unroll
@@ -186,6 +191,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
         *reinterpret_cast<uint4*>(pxl + (gr * 2 + e) * kNtChunk + row * 16) = make_uint4(l[4 * e], l[4 * e + 1], l[4 * e + 2], l[4 * e + 3]);
       }
     }
+    s_xsq[half * kNtRows + row] = xsq;
     ready();
     for (int it = 0; it < q.steps; ++it) {
       const NsStep by = ns_step(q, k2);
@@ -208,10 +214,17 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
         __syncwarp();
       }
       wait();
+      // The diagonals of A and A^2, sums of squares of rows, are taken from FP32 sums: the tensor core's, rounded towards zero with every
+      // MMA, are all too small by a few 1e-7, and the iteration carries that on (4e-6 of the result for 128 rows)
+      const float xx = s_xsq[row] + s_xsq[kNtRows + row];
+      float asq = 0.f;
       if (cluster == 1) {
         for (int gr = half; gr < 8; gr += 2) {
           uint32_t d[16], h[8], l[8];
           tmem_ld16(trow + gr * 16, d);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (gr * 16 + e == row) d[e] = __float_as_uint(xx);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             float v[2];
@@ -220,6 +233,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
               const int c = gr * 16 + 2 * e + i;
               v[i] = (unsigned)(c - sub * q.small) < (unsigned)q.small ? __uint_as_float(d[2 * e + i]) * by.gram : 0.f;
             }
+            asq = fmaf(v[0], v[0], fmaf(v[1], v[1], asq));
             ns_split(v[0], v[1], h[e], l[e]);
           }
 #pragma unroll
@@ -233,6 +247,9 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
         for (int gr = half; gr < 8; gr += 2) {
           uint32_t d[16];
           tmem_ld16(trow + gr * 16, d);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (gr * 16 + e == row) d[e] = __float_as_uint(xx);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             *reinterpret_cast<uint4*>(pah + (gr * 4 + e) * kNtChunk + row * 16) = make_uint4(d[4 * e], d[4 * e + 1], d[4 * e + 2], d[4 * e + 3]);
@@ -270,7 +287,17 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
         }
         nt_fence_async();
         nt_cluster_sync();
+        for (int gr = half; gr < 8; gr += 2)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint4 h4 = *reinterpret_cast<const uint4*>(pah + (gr * 2 + e) * kNtChunk + row * 16);
+            const uint4 l4 = *reinterpret_cast<const uint4*>(pal + (gr * 2 + e) * kNtChunk + row * 16);
+            const uint32_t h[4] = {h4.x, h4.y, h4.z, h4.w}, l[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { const float2 a = ns_join(h[i], l[i]); asq = fmaf(a.x, a.x, fmaf(a.y, a.y, asq)); }
+          }
       }
+      s_asq[half * kNtRows + row] = asq;
       ready();
       // ---- A^2
       if (warp == 0) {
@@ -290,9 +317,13 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
         __syncwarp();
       }
       wait();
+      const float aa = s_asq[row] + s_asq[kNtRows + row];
       for (int gr = half; gr < 8; gr += 2) {
         uint32_t d[16];
         tmem_ld16(trow + kNtRows + gr * 16, d);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (gr * 16 + e == row) d[e] = __float_as_uint(aa);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint4* const sh = reinterpret_cast<uint4*>(pah + (gr * 2 + e) * kNtChunk + row * 16);
@@ -302,8 +333,13 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 a = ns_join(h[i], l[i]);
-            ns_split(fmaf(q.b, a.x, q.c * (__uint_as_float(d[e * 8 + 2 * i]) * kNsUnscale)),
-                     fmaf(q.b, a.y, q.c * (__uint_as_float(d[e * 8 + 2 * i + 1]) * kNsUnscale)), h[i], l[i]);
+            float p0 = fmaf(by.b, a.x, by.c * __uint_as_float(d[e * 8 + 2 * i])), p1 = fmaf(by.b, a.y, by.c * __uint_as_float(d[e * 8 + 2 * i + 1]));
+            const int c = gr * 16 + e * 8 + 2 * i;
+            if (c == (row & ~1)) {       // the diagonal is kept apart (muon_warp.cu)
+              s_diag[row] = row & 1 ? p1 : p0;
+              if (row & 1) p1 = 0.f; else p0 = 0.f;
+            }
+            ns_split(p0, p1, h[i], l[i]);
           }
           *sh = make_uint4(h[0], h[1], h[2], h[3]);
           *sl = make_uint4(l[0], l[1], l[2], l[3]);
@@ -330,6 +366,8 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
       }
       wait();
       const bool last = it + 1 == q.steps;
+      const float own = by.a + s_diag[row];
+      xsq = 0.f;
       if (last && !ok) atomicOr(s_word + 3, 1u);
       if (last) __syncthreads();
       const bool write = last && in && s_word[3] == 0u;
@@ -346,8 +384,9 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 x = ns_join(h[i], l[i]);
-            v[e * 8 + 2 * i] = fmaf(by.a, x.x, __uint_as_float(d[e * 8 + 2 * i]) * by.unscale);
-            v[e * 8 + 2 * i + 1] = fmaf(by.a, x.y, __uint_as_float(d[e * 8 + 2 * i + 1]) * by.unscale);
+            v[e * 8 + 2 * i] = fmaf(own, x.x, __uint_as_float(d[e * 8 + 2 * i]));
+            v[e * 8 + 2 * i + 1] = fmaf(own, x.y, __uint_as_float(d[e * 8 + 2 * i + 1]));
+            xsq = fmaf(v[e * 8 + 2 * i], v[e * 8 + 2 * i], fmaf(v[e * 8 + 2 * i + 1], v[e * 8 + 2 * i + 1], xsq));
             ns_split(v[e * 8 + 2 * i], v[e * 8 + 2 * i + 1], h[i], l[i]);
           }
           if (!last) {
@@ -383,6 +422,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
             }
         }
       }
+      s_xsq[half * kNtRows + row] = xsq;
       ready();
     }
   }

@@ -4,8 +4,8 @@
 //
 // Arithmetic: the iteration multiplies a small singular value by up to a^steps (485 with the usual coefficients), so operands of
 // eleven bits would put errors of tenths into an orthogonal matrix.  X, A and bA + cA^2 are held as binary16 pairs hi + lo
-// (22 bits; X, whose entries become small, scaled by 2^10, so that its absolute error stays below 3e-11), every product is hi hi + hi lo
-// + lo hi on the tensor cores with FP32 accumulation, and a X is added in FP32.  On Gaussian matrices the result
+// (22 bits; X and A, whose entries become small, scaled by 2^10, so that their absolute error stays below 3e-11), every product is
+// hi hi + hi lo + lo hi on the tensor cores with FP32 accumulation, and a X is added in FP32.  On Gaussian matrices the result
 // is then 1e-6 off 64-bit arithmetic, as near as an FP32 iteration comes (1.1e-6).
 #pragma once
 #include <type_traits>
@@ -60,18 +60,18 @@ __device__ __forceinline__ NsStart ns_start(float eps, float ss, float f) {
   }
   return s;
 }
-// the factors of one step for a matrix at 2^k, which then is at the new k: A = gram * (product of the scaled X), P = b A + c A^2,
-// scaled X <- a X + P X
+// the factors of one step for a matrix at 2^k, which then is at the new k: scaled A = gram * (product of the scaled X), P = b (scaled A)
+// + c (scaled A)^2, scaled X <- a X + P X
 struct NsStep { float gram, a, b, c; };
 template <typename Q>
 __device__ __forceinline__ NsStep ns_step(const Q& q, int& k) {
   NsStep s;
-  s.gram = k > 50 ? 0.f : ns_exp2i(-20 - 2 * k);
+  s.gram = k > 50 ? 0.f : ns_exp2i(-10 - 2 * k);
   const int fall = min(k, k >= 4 ? q.far : q.near);
   const float r = ns_exp2i(-fall);
   s.a = q.a * r;
-  s.b = q.b * r;
-  s.c = q.c * r;
+  s.b = q.b * (r / kNsScale);
+  s.c = q.c * (r / (kNsScale * kNsScale));
   k -= fall;
   return s;
 }

@@ -1,6 +1,6 @@
 // Newton-Schulz iteration of small matrices (at most 32 x 96: the layers of a primitive), a warp per tile of 16 or 32 rows.
 //
-// X lies in the warp's shared memory as two binary16 matrices, A and bA + cA^2 in its registers as fragments of m16n8 tiles (lane
+// X lies in the warp's shared memory as binary16 pairs, in panels of 16 columns, A and bA + cA^2 in its registers as fragments of m16n8 tiles (lane
 // 4 g + t: rows g and g + 8, columns 2 t and 2 t + 1), in which form a symmetric matrix is at once an A and a B operand.  ldmatrix gives X
 // as the A operand of X X^T, whose words are also its B operand, and, transposed, as the B operand of (bA + cA^2) X.  Of A and A^2 the
 // 16 x 16 blocks on and below the diagonal are computed, the others are their transposes (movmatrix).  Several matrices of few rows
@@ -18,6 +18,11 @@ namespace mlpsp {
 __device__ __forceinline__ void ns_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same onto nothing
+__device__ __forceinline__ void ns_mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void ns_mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
@@ -46,24 +51,13 @@ __device__ __forceinline__ void ns_stmatrix(uint32_t addr, const uint32_t (&r)[4
   else asm volatile("stmatrix.sync.aligned.m8n8.x2.shared.b16 [%0], {%1, %2};" ::"r"(addr), "r"(r[0]), "r"(r[1]) : "memory");
 }
 
-// two FP32 operations in one instruction
-__device__ __forceinline__ float2 ns_fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)),
-      "l"(reinterpret_cast<const unsigned long long&>(b)), "l"(reinterpret_cast<const unsigned long long&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 ns_mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<const unsigned long long&>(a)),
-      "l"(reinterpret_cast<const unsigned long long&>(b)));
-  return d;
-}
-__device__ __forceinline__ float2 ns_both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ void ns_split2(float2 x, uint32_t& hi, uint32_t& lo) {
-  hi = pack_h2<false>(x.x, x.y);
-  const float2 r = ns_fma2(ns_unpack<false>(hi), ns_both(-1.f), x);
-  lo = pack_h2<false>(r.x, r.y);
+// ns_split on the integer and FP32 units: FP32 halves come back from binary16 on half of the multiply-add units only, which were as busy
+// as the tensor cores with ns_split's.  hi: x with its lowest 13 bits rounded off, which binary16 holds exactly down to 2^-14.
+__device__ __forceinline__ float ns_head(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); }
+__device__ __forceinline__ void ns_split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  const float h0 = ns_head(x0), h1 = ns_head(x1);
+  hi = pack_h2<false>(h0, h1);
+  lo = pack_h2<false>(x0 - h0, x1 - h1);
 }
 
 // fragments of a symmetric [16 MB x 16 MB] matrix: f[mb][n][h] = rows 16 mb + 8 h + g, columns 8 n + 2 t and + 1
@@ -85,7 +79,7 @@ __device__ __forceinline__ void ns_mirror(NsFrag<MB>& s) {
 // d += x x^T over 8 K columns; x.. as ns_ldmatrix<K> gives them; block (mb, n), n <= 2 mb + 1, is d[mb (mb + 1) + n].  The blocks
 // advance together, since an MMA takes four times as long to answer as to issue; small products first, so that the tensor core's
 // rounding of a sum towards zero meets fewer large ones.
-template <int MB, int K>
+template <int MB, int K, bool FIRST>
 __device__ __forceinline__ void ns_gram(const uint32_t (&hi)[MB][4], const uint32_t (&lo)[MB][4], float (&d)[MB * (MB + 1)][4]) {
 #pragma unroll
   for (int part = 0; part < 3; ++part) {
@@ -95,21 +89,22 @@ __device__ __forceinline__ void ns_gram(const uint32_t (&hi)[MB][4], const uint3
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int n = 0; n < 2 * mb + 2; ++n) {
-        if (K == 2) ns_mma(d[mb * (mb + 1) + n], l[mb][0], l[mb][1], l[mb][2], l[mb][3], r[n >> 1][n & 1], r[n >> 1][2 + (n & 1)]);
+        if (K == 2 && FIRST && part == 0) ns_mma_first(d[mb * (mb + 1) + n], l[mb][0], l[mb][1], l[mb][2], l[mb][3], r[n >> 1][n & 1], r[n >> 1][2 + (n & 1)]);
+        else if (K == 2) ns_mma(d[mb * (mb + 1) + n], l[mb][0], l[mb][1], l[mb][2], l[mb][3], r[n >> 1][n & 1], r[n >> 1][2 + (n & 1)]);
         else ns_mma8(d[mb * (mb + 1) + n], l[mb][0], l[mb][1], r[n >> 1][n & 1]);
       }
   }
 }
 
-template <int MB, int NB> __host__ __device__ constexpr int ns_row_bytes() { return (NB | 1) * 16; }      // an odd number of 16-byte units: no bank conflicts
-template <int MB, int NB> __host__ __device__ constexpr int ns_warp_smem() { return 2 * 16 * MB * ns_row_bytes<MB, NB>(); }
+// A panel: hi [16 MB rows][16 columns], then lo; the two 16-byte halves of a row change places every four rows, so that eight rows of
+// one half lie in different banks.  It takes the bytes of its values in FP32, as which they arrive.
+template <int MB> __host__ __device__ constexpr int ns_panel_bytes() { return 16 * MB * 64; }
+template <int MB, int NB> __host__ __device__ constexpr int ns_warp_smem() { return (NB + 1) / 2 * ns_panel_bytes<MB>(); }
 
 template <int MB, int NB, int CTAS>
 __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int pack, const int64_t tiles) {
   constexpr int KH = MB == 1 ? 2 : 1;       // with one block of rows, rows h = 0 and 1 of a lane may belong to two matrices
-  constexpr int CH = MB == 2 ? (NB % 3 == 0 ? 3 : 4) : (NB % 3 == 0 ? 6 > NB ? NB : NB % 6 == 0 ? 6 : 9 : 4);
-  static_assert(NB % CH == 0, "whole chunks");
-  constexpr int kRow = ns_row_bytes<MB, NB>(), kLo = 16 * MB * kRow;
+  constexpr int kPanels = (NB + 1) / 2, kPanel = ns_panel_bytes<MB>(), kLo = kPanel / 2, kBlock = 16 * 32;
   extern __shared__ __align__(128) char smem[];
   chain_wait();
   chain_release();
@@ -117,7 +112,8 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
   char* const mine = smem + (threadIdx.x >> 5) * ns_warp_smem<MB, NB>();
   const uint32_t xs = smem_u32(mine);
   // this lane's row of the 8 x 8 blocks that ldmatrix and stmatrix name: lanes 0-7 rows 0-7, 8-15 rows 8-15, 16-31 the same, 8 columns on
-  const uint32_t xa = xs + (lane & 15) * kRow + (lane >> 4) * 16;
+  const uint32_t xa = xs + (lane & 15) * 32 + (((lane >> 4) ^ ((lane >> 2) & 1)) << 4);
+  float2* const keep = reinterpret_cast<float2*>(mine) + lane;      // this lane's values of a panel in FP32: [2 columns of blocks][MB][2]
   // the matrix of the tile and its row, for this lane's rows; which columns of A belong to the same matrix
   int sub[KH], row[KH];
   uint32_t same = 0u;      // bit h * 4 + n * 2 + e
@@ -146,49 +142,48 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
     auto in = [&](int mb, int h) { return on[h % KH] && (MB == 1 || mb * 16 + h * 8 + g < q.small); };
     auto base = [&](int mb, int h) { return MB == 1 ? first[h % KH] : first[0] + (int64_t)((mb * 16 + h * 8) * q.rs); };
     __syncwarp();
-    float2 x[MB][NB][2];
+    // ---- gradient and momentum, a panel at a time, to this lane's places in shared memory; sums of squares on the way
+    float squares[2] = {0.f, 0.f};
+    auto fetch = [&](auto tag, auto step) {
+      constexpr int TYPE = decltype(tag)::value;
+      constexpr bool STEP = decltype(step)::value;
+#pragma unroll 1
+      for (int p = 0; p < kPanels; ++p) {
+        NsVec<2> v[2][MB][2], m[2][MB][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int col = p * 16 + u * 8 + 2 * t;
+              v[u][mb][h] = m[u][mb][h] = NsVec<2>{{0.f, 0.f}};
+              if (in(mb, h) && col < q.large) {
+                v[u][mb][h] = ns_load<2>(q.g, base(mb, h) + col, TYPE);
+                if (STEP) m[u][mb][h] = ns_load<2>(q.m, base(mb, h) + col, MLPSP_PRECISION_F32);
+              }
+            }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int col = p * 16 + u * 8 + 2 * t;
+              float2 y = make_float2(v[u][mb][h].v[0], v[u][mb][h].v[1]);
+              if (STEP) {
+                NsVec<2> n = m[u][mb][h];
+                n.v[0] = ns_new_momentum(q, y.x, n.v[0]);
+                n.v[1] = ns_new_momentum(q, y.y, n.v[1]);
+                y = make_float2(ns_update(q, y.x, n.v[0]), ns_update(q, y.y, n.v[1]));
+                if (in(mb, h) && col < q.large) ns_store<2>(q.m, base(mb, h) + col, MLPSP_PRECISION_F32, n);
+              }
+              squares[h] = fmaf(y.x, y.x, fmaf(y.y, y.y, squares[h]));
+              keep[(p * 2 * MB * 2 + (u * MB + mb) * 2 + h) * 32] = y;
+            }
+      }
+    };
     if (q.vec >= 2) {
-      auto fetch = [&](auto tag, auto step) {
-        constexpr int TYPE = decltype(tag)::value;
-        constexpr bool STEP = decltype(step)::value;
-        // a few columns of blocks at a time, so that their loads are under way together
-#pragma unroll
-        for (int c0 = 0; c0 < NB; c0 += CH) {
-          NsVec<2> v[MB][CH][2], m[MB][CH][2];
-#pragma unroll
-          for (int u = 0; u < CH; ++u)
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int col = (c0 + u) * 8 + 2 * t;
-                v[mb][u][h] = m[mb][u][h] = NsVec<2>{{0.f, 0.f}};
-                if (in(mb, h) && col < q.large) {
-                  v[mb][u][h] = ns_load<2>(q.g, base(mb, h) + col, TYPE);
-                  if (STEP) m[mb][u][h] = ns_load<2>(q.m, base(mb, h) + col, MLPSP_PRECISION_F32);
-                }
-              }
-#pragma unroll
-          for (int u = 0; u < CH; ++u)
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int col = (c0 + u) * 8 + 2 * t;
-                float y[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  y[e] = v[mb][u][h].v[e];
-                  if (STEP) {
-                    m[mb][u][h].v[e] = ns_new_momentum(q, y[e], m[mb][u][h].v[e]);
-                    y[e] = ns_update(q, y[e], m[mb][u][h].v[e]);
-                  }
-                }
-                x[mb][c0 + u][h] = make_float2(y[0], y[1]);
-                if (STEP && in(mb, h) && col < q.large) ns_store<2>(q.m, base(mb, h) + col, MLPSP_PRECISION_F32, m[mb][u][h]);
-              }
-        }
-      };
       if (q.m) {
         if (q.type == MLPSP_PRECISION_F32) fetch(NsTag<MLPSP_PRECISION_F32>{}, NsTag<1>{});
         else if (q.type == MLPSP_PRECISION_F16) fetch(NsTag<MLPSP_PRECISION_F16>{}, NsTag<1>{});
@@ -199,36 +194,29 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
         else fetch(NsTag<MLPSP_PRECISION_BF16>{}, NsTag<0>{});
       }
     } else {
-      // odd rows, transposed matrices: element by element, through this lane's own places in shared memory so that the loop stays rolled
-      float2* const keep = reinterpret_cast<float2*>(mine) + lane;
+      // odd rows, transposed matrices: element by element
 #pragma unroll 1
-      for (int nb = 0; nb < NB; ++nb)
+      for (int i = 0; i < kPanels * 2 * MB; ++i) {
+        const int nb = i / MB, mb = i % MB;
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
+        for (int h = 0; h < 2; ++h) {
+          float y[2] = {0.f, 0.f};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float y[2] = {0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int col = nb * 8 + 2 * t + e;
-              if (!in(mb, h) || col >= q.large) continue;
-              const int64_t at = base(mb, h) + (int64_t)col * q.cs;
-              y[e] = ns_load<1>(q.g, at, q.type).v[0];
-              if (q.m) {
-                const float m = ns_new_momentum(q, y[e], q.m[at]);
-                y[e] = ns_update(q, y[e], m);
-                q.m[at] = m;
-              }
+          for (int e = 0; e < 2; ++e) {
+            const int col = nb * 8 + 2 * t + e;
+            if (!in(mb, h) || col >= q.large) continue;
+            const int64_t at = base(mb, h) + (int64_t)col * q.cs;
+            y[e] = ns_load<1>(q.g, at, q.type).v[0];
+            if (q.m) {
+              const float m = ns_new_momentum(q, y[e], q.m[at]);
+              y[e] = ns_update(q, y[e], m);
+              q.m[at] = m;
             }
-            keep[((nb * MB + mb) * 2 + h) * 32] = make_float2(y[0], y[1]);
           }
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) x[mb][nb][h] = keep[((nb * MB + mb) * 2 + h) * 32];
-      __syncwarp();
+          squares[h] = fmaf(y[0], y[0], fmaf(y[1], y[1], squares[h]));
+          keep[(i * 2 + h) * 32] = make_float2(y[0], y[1]);
+        }
+      }
     }
     // Frobenius norms, per matrix of the tile; once more, scaled, where the squares leave the range of FP32
     float f[KH];
@@ -237,17 +225,18 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
     for (int h = 0; h < KH; ++h) f[h] = 1.f;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
-      float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+      if (pass == 1) {
+        squares[0] = squares[1] = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < kPanels * 2 * MB; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 v = ns_mul2(x[mb][nb][h], ns_both(f[h % KH]));
-            s2[h] = ns_fma2(v, v, s2[h]);
+            const float2 v = keep[(i * 2 + h) * 32];
+            const float v0 = v.x * f[h % KH], v1 = v.y * f[h % KH];
+            squares[h] = fmaf(v0, v0, fmaf(v1, v1, squares[h]));
           }
-      float ss[2] = {s2[0].x + s2[0].y, s2[1].x + s2[1].y};
+      }
+      float ss[2] = {squares[0], squares[1]};
       if (pack == 1) {
         float s = ss[0] + ss[1];
 #pragma unroll
@@ -281,29 +270,44 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
       if (!__any_sync(0xffffffffu, again)) break;
     }
     int k2[KH];
-    bool lost[KH];
+    float done[KH];          // what the scaled result is multiplied by at the end, but for 2^-k
+    bool odd = false;
 #pragma unroll
-    for (int h = 0; h < KH; ++h) { k2[h] = start[h].k; lost[h] = start[h].lost; }
+    for (int h = 0; h < KH; ++h) {
+      k2[h] = start[h].k;
+      done[h] = start[h].lost ? __int_as_float(0x7fffffff) : 1.f / kNsScale;
+      odd |= start[h].lost || start[h].pre != 1.f;
+    }
+    if (__any_sync(0xffffffffu, odd))
+#pragma unroll 1
+      for (int i = 0; i < kPanels * 2 * MB; ++i)
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
+        for (int h = 0; h < 2; ++h) {
+          float2& v = keep[(i * 2 + h) * 32];
+          const NsStart& s = start[h % KH];
+          v = s.lost ? make_float2(0.f, 0.f) : make_float2(v.x * s.pre, v.y * s.pre);
+        }
+    // ---- X0, panel by panel in place
+#pragma unroll 1
+    for (int p = 0; p < kPanels; ++p) {
+      uint32_t hi[MB][4], lo[MB][4];
 #pragma unroll
-      for (int nb = 0; nb < NB; nb += 2) {
-        constexpr int kTail = NB & 1;
-        uint32_t hi[4] = {0u, 0u, 0u, 0u}, lo[4] = {0u, 0u, 0u, 0u};
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (nb + u < NB)
+        for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const NsStart& s = start[h % KH];
-              float2 v = ns_mul2(ns_mul2(x[mb][(nb + u) % NB][h], ns_both(s.pre)), ns_both(s.inv));
-              if (s.lost) v = make_float2(0.f, 0.f);
-              ns_split2(v, hi[2 * u + h], lo[2 * u + h]);
-            }
-        const uint32_t at = xa + mb * 16 * kRow + nb * 16;
-        if (kTail && nb + 1 == NB) { ns_stmatrix<1>(at, hi); ns_stmatrix<1>(at + kLo, lo); }
-        else { ns_stmatrix<2>(at, hi); ns_stmatrix<2>(at + kLo, lo); }
+          for (int h = 0; h < 2; ++h) {
+            const float2 v = keep[(p * 2 * MB * 2 + (u * MB + mb) * 2 + h) * 32];
+            const float s = start[h % KH].inv;
+            ns_split2(v.x * s, v.y * s, hi[mb][2 * u + h], lo[mb][2 * u + h]);
+          }
+      __syncwarp();
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        ns_stmatrix<2>(xa + p * kPanel + mb * kBlock, hi[mb]);
+        ns_stmatrix<2>(xa + p * kPanel + mb * kBlock + kLo, lo[mb]);
       }
+    }
     __syncwarp();
 #pragma unroll 1
     for (int it = 0; it < q.steps; ++it) {
@@ -311,45 +315,43 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
 #pragma unroll
       for (int h = 0; h < KH; ++h) by[h] = ns_step(q, k2[h]);
       float d[MB * (MB + 1)][4];
-      auto clear = [&] {
-#pragma unroll
-        for (int i = 0; i < MB * (MB + 1); ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
-      };
       // ---- A = X X^T
-      clear();
-      auto columns = [&](int nb, auto width) {
+#pragma unroll
+      for (int i = 0; i < MB * (MB + 1); ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
+      auto columns = [&](int p, auto width) {
         constexpr int K = decltype(width)::value;
         uint32_t hi[MB][4], lo[MB][4];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-          ns_ldmatrix<K, false>(hi[mb], xa + mb * 16 * kRow + nb * 16);
-          ns_ldmatrix<K, false>(lo[mb], xa + mb * 16 * kRow + nb * 16 + kLo);
+          ns_ldmatrix<K, false>(hi[mb], xa + p * kPanel + mb * kBlock);
+          ns_ldmatrix<K, false>(lo[mb], xa + p * kPanel + mb * kBlock + kLo);
         }
-        ns_gram<MB, K>(hi, lo, d);
+        ns_gram<MB, K, false>(hi, lo, d);
       };
 #pragma unroll 1
-      for (int nb = 0; nb + 1 < NB; nb += 2) columns(nb, NsTag<2>{});
-      if (NB & 1) columns(NB - 1, NsTag<1>{});
+      for (int p = 0; p < NB / 2; ++p) columns(p, NsTag<2>{});
+      if (NB & 1) columns(NB / 2, NsTag<1>{});
       NsFrag<MB> A;
+      float a32[MB * (MB + 1)][4];
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int n = 0; n < 2 * mb + 2; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float(&o)[4] = d[mb * (mb + 1) + n];
-            float2 v = ns_mul2(make_float2(o[2 * h], o[2 * h + 1]), ns_both(by[h % KH].gram));
-            if (MB == 1) {
-              if (!(same >> (h * 4 + n * 2) & 1u)) v.x = 0.f;
-              if (!(same >> (h * 4 + n * 2 + 1) & 1u)) v.y = 0.f;
+            const int i = mb * (mb + 1) + n;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v = d[i][2 * h + e] * by[h % KH].gram;
+              if (MB == 1 && !(same >> (h * 4 + n * 2 + e) & 1u)) v = 0.f;
+              a32[i][2 * h + e] = v;
             }
-            ns_split2(v, A.hi[mb][n][h], A.lo[mb][n][h]);
+            ns_split2(a32[i][2 * h], a32[i][2 * h + 1], A.hi[mb][n][h], A.lo[mb][n][h]);
           }
       ns_mirror<MB>(A);
-      float diag[MB][2];
+      float own[MB][2];        // a + P(r, r) of this lane's rows
       // ---- P = b A + c A^2.  Its diagonal is kept apart and multiplies X in FP32 below: the rest is smaller, and with it what the tensor
       // core's rounding towards zero takes off (4e-6 of the result for 128 rows with the diagonal in, 2e-6 so)
-      clear();
 #pragma unroll
       for (int k = 0; k < MB; ++k) {
         uint32_t hi[MB][4], lo[MB][4];
@@ -357,7 +359,8 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
         for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
           for (int i = 0; i < 4; ++i) { hi[mb][i] = A.hi[mb][2 * k + (i >> 1)][i & 1]; lo[mb][i] = A.lo[mb][2 * k + (i >> 1)][i & 1]; }
-        ns_gram<MB, 2>(hi, lo, d);
+        if (k == 0) ns_gram<MB, 2, true>(hi, lo, d);
+        else ns_gram<MB, 2, false>(hi, lo, d);
       }
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
@@ -365,36 +368,35 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
         for (int n = 0; n < 2 * mb + 2; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float(&o)[4] = d[mb * (mb + 1) + n];
+            const int i = mb * (mb + 1) + n;
             const NsStep& s = by[h % KH];
-            float2 v = ns_mul2(make_float2(o[2 * h], o[2 * h + 1]), ns_both(s.c));
-            v = ns_fma2(ns_unpack<false>(A.lo[mb][n][h]), ns_both(s.b), v);
-            v = ns_fma2(ns_unpack<false>(A.hi[mb][n][h]), ns_both(s.b), v);
+            float v0 = fmaf(s.b, a32[i][2 * h], s.c * d[i][2 * h]), v1 = fmaf(s.b, a32[i][2 * h + 1], s.c * d[i][2 * h + 1]);
             if (n == 2 * mb + h) {       // the block on the diagonal: lane 4 g + g / 2 has row g's element
-              diag[mb][h] = g & 1 ? v.y : v.x;
-              if (2 * t == g) v.x = 0.f;
-              if (2 * t + 1 == g) v.y = 0.f;
+              own[mb][h] = s.a + __shfl_sync(0xffffffffu, g & 1 ? v1 : v0, 4 * g + (g >> 1));
+              if (2 * t == g) v0 = 0.f;
+              if (2 * t + 1 == g) v1 = 0.f;
             }
-            ns_split2(v, A.hi[mb][n][h], A.lo[mb][n][h]);
+            ns_split2(v0, v1, A.hi[mb][n][h], A.lo[mb][n][h]);
           }
       ns_mirror<MB>(A);
-      float2 own[MB][2];       // a + P(r, r) of this lane's rows
+      // The diagonal blocks of P's head with a + P(r, r) in binary16 on the diagonal, for the product with X's low half: what that adds
+      // of (a + P(r, r)) X is right to 2^-11 of the low half, so only X's head is left to be multiplied below.
+      uint32_t mixed[MB][2];
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) own[mb][h] = ns_both(by[h % KH].a + __shfl_sync(0xffffffffu, diag[mb][h], 4 * g + (g >> 1)));
+        for (int h = 0; h < 2; ++h)
+          mixed[mb][h] = A.hi[mb][2 * mb + h][h] | (2 * t == (g & ~1) ? pack_h2<false>(g & 1 ? 0.f : own[mb][h], g & 1 ? own[mb][h] : 0.f) : 0u);
       // ---- X <- a X + P X, two blocks of eight columns at a time
       const bool last = it + 1 == q.steps;
-      auto advance = [&](int nb, auto width) {
+      auto advance = [&](int p, auto width) {
         constexpr int N = decltype(width)::value;
         uint32_t bh[MB][4], bl[MB][4];
         float e[MB][N][4];
 #pragma unroll
         for (int k = 0; k < MB; ++k) {
-          ns_ldmatrix<N, true>(bh[k], xa + k * 16 * kRow + nb * 16);
-          ns_ldmatrix<N, true>(bl[k], xa + k * 16 * kRow + nb * 16 + kLo);
-#pragma unroll
-          for (int n = 0; n < N; ++n) e[k][n][0] = e[k][n][1] = e[k][n][2] = e[k][n][3] = 0.f;
+          ns_ldmatrix<N, true>(bh[k], xa + p * kPanel + k * kBlock);
+          ns_ldmatrix<N, true>(bl[k], xa + p * kPanel + k * kBlock + kLo);
         }
 #pragma unroll
         for (int part = 0; part < 3; ++part) {
@@ -405,40 +407,42 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-              for (int mb = 0; mb < MB; ++mb)
-                ns_mma(e[mb][n], l[mb][2 * k][0], l[mb][2 * k][1], l[mb][2 * k + 1][0], l[mb][2 * k + 1][1], r[k][2 * n], r[k][2 * n + 1]);
+              for (int mb = 0; mb < MB; ++mb) {
+                const uint32_t a0 = part == 0 && k == mb ? mixed[mb][0] : l[mb][2 * k][0], a3 = part == 0 && k == mb ? mixed[mb][1] : l[mb][2 * k + 1][1];
+                if (part == 0 && k == 0) ns_mma_first(e[mb][n], a0, l[mb][0][1], l[mb][1][0], a3, r[0][2 * n], r[0][2 * n + 1]);
+                else ns_mma(e[mb][n], a0, l[mb][2 * k][1], l[mb][2 * k + 1][0], a3, r[k][2 * n], r[k][2 * n + 1]);
+              }
         }
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-          const uint32_t at = xa + mb * 16 * kRow + nb * 16;
+          const uint32_t at = xa + p * kPanel + mb * kBlock;
           uint32_t hi[4], lo[4];
           ns_ldmatrix<N, false>(hi, at);
-          ns_ldmatrix<N, false>(lo, at + kLo);
-          float2 v[N][2];
+          float v[N][2][2];
 #pragma unroll
           for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              v[n][h] = ns_fma2(ns_unpack<false>(lo[2 * n + h]), own[mb][h], make_float2(e[mb][n][2 * h], e[mb][n][2 * h + 1]));
-              v[n][h] = ns_fma2(ns_unpack<false>(hi[2 * n + h]), own[mb][h], v[n][h]);
-              ns_split2(v[n][h], hi[2 * n + h], lo[2 * n + h]);
+              const float2 x = ns_unpack<false>(hi[2 * n + h]);
+              v[n][h][0] = fmaf(own[mb][h], x.x, e[mb][n][2 * h]);
+              v[n][h][1] = fmaf(own[mb][h], x.y, e[mb][n][2 * h + 1]);
+              ns_split2(v[n][h][0], v[n][h][1], hi[2 * n + h], lo[2 * n + h]);
             }
           if (!last) {
             ns_stmatrix<N>(at, hi);
             ns_stmatrix<N>(at + kLo, lo);
             continue;
           }
-          const float nan = __int_as_float(0x7fffffff);
 #pragma unroll
           for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int col = (nb + n) * 8 + 2 * t;
+              const int col = p * 16 + n * 8 + 2 * t;
               if (!in(mb, h) || col >= q.large) continue;
-              const float fin = ns_exp2i(-10 - k2[h % KH]);
+              const float fin = done[h % KH] * ns_exp2i(-k2[h % KH]);
               NsVec<2> y;
-              y.v[0] = lost[h % KH] ? nan : v[n][h].x * fin;
-              y.v[1] = lost[h % KH] ? nan : v[n][h].y * fin;
+              y.v[0] = v[n][h][0] * fin;
+              y.v[1] = v[n][h][1] * fin;
               if (q.vec >= 2) {
                 const int64_t i = base(mb, h) + col;
                 if (q.m) {
@@ -460,8 +464,8 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
         }
       };
 #pragma unroll 1
-      for (int nb = 0; nb + 1 < NB; nb += 2) advance(nb, NsTag<2>{});
-      if (NB & 1) advance(NB - 1, NsTag<1>{});
+      for (int p = 0; p < NB / 2; ++p) advance(p, NsTag<2>{});
+      if (NB & 1) advance(NB / 2, NsTag<1>{});
       __syncwarp();
     }
   }
@@ -482,8 +486,8 @@ static int ns_warp(const NsArgs& q, cudaStream_t st) {
 
 int launch_ns_warp(const NsArgs& q, cudaStream_t st) {
   const int nb = (q.large + 7) / 8;
-  if (q.small <= 16) return nb <= 4 ? ns_warp<1, 4, 6>(q, st) : nb <= 6 ? ns_warp<1, 6, 6>(q, st) : nb <= 9 ? ns_warp<1, 9, 5>(q, st) : ns_warp<1, 12, 5>(q, st);
-  return nb <= 4 ? ns_warp<2, 4, 4>(q, st) : nb <= 6 ? ns_warp<2, 6, 4>(q, st) : nb <= 9 ? ns_warp<2, 9, 4>(q, st) : ns_warp<2, 12, 3>(q, st);
+  if (q.small <= 16) return nb <= 4 ? ns_warp<1, 4, 8>(q, st) : nb <= 6 ? ns_warp<1, 6, 7>(q, st) : nb <= 9 ? ns_warp<1, 9, 7>(q, st) : ns_warp<1, 12, 7>(q, st);
+  return nb <= 4 ? ns_warp<2, 4, 5>(q, st) : nb <= 6 ? ns_warp<2, 6, 5>(q, st) : nb <= 9 ? ns_warp<2, 9, 5>(q, st) : ns_warp<2, 12, 4>(q, st);
 }
 
 }  // namespace mlpsp

@@ -76,22 +76,26 @@ __device__ __forceinline__ void ns_mirror(NsFrag<MB>& s) {
       }
 }
 
-// d += x x^T over 8 K columns; x.. as ns_ldmatrix<K> gives them; block (mb, n), n <= 2 mb + 1, is d[mb (mb + 1) + n].  The blocks
+// d += x x^T over 8 K columns; block (mb, n), n <= 2 mb + 1, is d[mb (mb + 1) + n].  ah, al: x as ns_ldmatrix<K> gives it; bh, bl: the
+// same words with those of a row next to each other, as B operands want them (K = 1: the same).  The blocks
 // advance together, since an MMA takes four times as long to answer as to issue; small products first, so that the tensor core's
 // rounding of a sum towards zero meets fewer large ones.
 template <int MB, int K, bool FIRST>
-__device__ __forceinline__ void ns_gram(const uint32_t (&hi)[MB][4], const uint32_t (&lo)[MB][4], float (&d)[MB * (MB + 1)][4]) {
+__device__ __forceinline__ void ns_gram(const uint32_t (&ah)[MB][4], const uint32_t (&al)[MB][4], const uint32_t (&bh)[MB][4],
+                                        const uint32_t (&bl)[MB][4], float (&d)[MB * (MB + 1)][4]) {
 #pragma unroll
   for (int part = 0; part < 3; ++part) {
-    const auto& l = part == 1 ? lo : hi;
-    const auto& r = part == 0 ? lo : hi;
+    const auto& l = part == 1 ? al : ah;
+    const auto& r = part == 0 ? bl : bh;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int n = 0; n < 2 * mb + 2; ++n) {
-        if (K == 2 && FIRST && part == 0) ns_mma_first(d[mb * (mb + 1) + n], l[mb][0], l[mb][1], l[mb][2], l[mb][3], r[n >> 1][n & 1], r[n >> 1][2 + (n & 1)]);
-        else if (K == 2) ns_mma(d[mb * (mb + 1) + n], l[mb][0], l[mb][1], l[mb][2], l[mb][3], r[n >> 1][n & 1], r[n >> 1][2 + (n & 1)]);
-        else ns_mma8(d[mb * (mb + 1) + n], l[mb][0], l[mb][1], r[n >> 1][n & 1]);
+        float(&o)[4] = d[mb * (mb + 1) + n];
+        const uint32_t(&w)[4] = r[n >> 1];
+        if (K == 1) ns_mma8(o, l[mb][0], l[mb][1], w[n & 1]);
+        else if (FIRST && part == 0) ns_mma_first(o, l[mb][0], l[mb][1], l[mb][2], l[mb][3], w[2 * (n & 1)], w[2 * (n & 1) + 1]);
+        else ns_mma(o, l[mb][0], l[mb][1], l[mb][2], l[mb][3], w[2 * (n & 1)], w[2 * (n & 1) + 1]);
       }
   }
 }
@@ -113,6 +117,8 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
   const uint32_t xs = smem_u32(mine);
   // this lane's row of the 8 x 8 blocks that ldmatrix and stmatrix name: lanes 0-7 rows 0-7, 8-15 rows 8-15, 16-31 the same, 8 columns on
   const uint32_t xa = xs + (lane & 15) * 32 + (((lane >> 4) ^ ((lane >> 2) & 1)) << 4);
+  // the same with the two halves of a row one after the other: lanes 0-7 rows 0-7, 8-15 the same, 8 columns on, 16-31 rows 8-15
+  const uint32_t xb = xs + ((lane & 7) + ((lane >> 4) << 3)) * 32 + ((((lane >> 3) & 1) ^ ((lane >> 2) & 1)) << 4);
   float2* const keep = reinterpret_cast<float2*>(mine) + lane;      // this lane's values of a panel in FP32: [2 columns of blocks][MB][2]
   // the matrix of the tile and its row, for this lane's rows; which columns of A belong to the same matrix
   int sub[KH], row[KH];
@@ -320,13 +326,19 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
       for (int i = 0; i < MB * (MB + 1); ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
       auto columns = [&](int p, auto width) {
         constexpr int K = decltype(width)::value;
-        uint32_t hi[MB][4], lo[MB][4];
+        uint32_t hi[MB][4], lo[MB][4], bh[MB][4], bl[MB][4];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
-          ns_ldmatrix<K, false>(hi[mb], xa + p * kPanel + mb * kBlock);
-          ns_ldmatrix<K, false>(lo[mb], xa + p * kPanel + mb * kBlock + kLo);
+          const int at = p * kPanel + mb * kBlock;
+          ns_ldmatrix<K, false>(hi[mb], xa + at);
+          ns_ldmatrix<K, false>(lo[mb], xa + at + kLo);
+          if (K == 2) {
+            ns_ldmatrix<K, false>(bh[mb], xb + at);
+            ns_ldmatrix<K, false>(bl[mb], xb + at + kLo);
+          }
         }
-        ns_gram<MB, K, false>(hi, lo, d);
+        if (K == 2) ns_gram<MB, K, false>(hi, lo, bh, bl, d);
+        else ns_gram<MB, K, false>(hi, lo, hi, lo, d);
       };
 #pragma unroll 1
       for (int p = 0; p < NB / 2; ++p) columns(p, NsTag<2>{});
@@ -354,13 +366,18 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
       // core's rounding towards zero takes off (4e-6 of the result for 128 rows with the diagonal in, 2e-6 so)
 #pragma unroll
       for (int k = 0; k < MB; ++k) {
-        uint32_t hi[MB][4], lo[MB][4];
+        uint32_t hi[MB][4], lo[MB][4], bh[MB][4], bl[MB][4];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { hi[mb][i] = A.hi[mb][2 * k + (i >> 1)][i & 1]; lo[mb][i] = A.lo[mb][2 * k + (i >> 1)][i & 1]; }
-        if (k == 0) ns_gram<MB, 2, true>(hi, lo, d);
-        else ns_gram<MB, 2, false>(hi, lo, d);
+          for (int i = 0; i < 4; ++i) {
+            hi[mb][i] = A.hi[mb][2 * k + (i >> 1)][i & 1];
+            lo[mb][i] = A.lo[mb][2 * k + (i >> 1)][i & 1];
+            bh[mb][i] = A.hi[mb][2 * k + (i & 1)][i >> 1];
+            bl[mb][i] = A.lo[mb][2 * k + (i & 1)][i >> 1];
+          }
+        if (k == 0) ns_gram<MB, 2, true>(hi, lo, bh, bl, d);
+        else ns_gram<MB, 2, false>(hi, lo, bh, bl, d);
       }
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)

@@ -458,13 +458,21 @@ int mlpsp_weight_gradients(const mlpsp_scene* scene, const int64_t* offsets, con
 int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols);
 int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a, double b,
                         double c, double eps, void* out, int32_t* status, void* stream);
-/* One step, in place, on n weight matrices and their momenta (FP32): m <- m + (1 - momentum)(g - m), U = g + momentum (m - g)
- * (nesterov) or m, w <- (1 - lr weight_decay) w - lr scale X(U), X as above.  grads [n, rows, cols] of grad_dtype.
- * active [n] (bytes, or NULL): matrices whose byte is zero keep weights and momenta and are not read.  The four arrays may not
- * overlap. */
-int mlpsp_muon_step(float* weights, const void* grads, int32_t grad_dtype, float* momenta, const uint8_t* active, int64_t n, int32_t rows,
-                    int32_t cols, double lr, double momentum, int32_t nesterov, double weight_decay, double scale, int32_t steps,
-                    double a, double b, double c, double eps, int32_t* status, void* stream);
+/* One step, in place, on the weight matrices of `count` tensors and their momenta (FP32): m <- m + (1 - momentum)(g - m),
+ * U = g + momentum (m - g) (nesterov) or m, w <- (1 - lr weight_decay) w - lr scale X(U), X as above.
+ * active [n] (bytes, or NULL; then every tensor's n is the same): matrices whose byte is zero keep weights and momenta and are not
+ * read.  No weights or momenta may overlap any other array of the call: the tensors' launches run side by side. */
+typedef struct mlpsp_muon_tensor {
+  float* weights;            /* [n, rows, cols] */
+  const void* grads;         /* the same, of grad_dtype (MLPSP_PRECISION_*) */
+  float* momenta;
+  int64_t n;
+  int32_t rows, cols;
+  double scale;              /* of the learning rate, e.g. sqrt(max(1, rows / cols)) */
+  int32_t grad_dtype, reserved0;
+} mlpsp_muon_tensor;
+int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, const uint8_t* active, double lr, double momentum, int32_t nesterov,
+                    double weight_decay, int32_t steps, double a, double b, double c, double eps, int32_t* status, void* stream);
 
 /* ---- the step after the feature map: feature decoder and text query ---- */
 

@@ -65,6 +65,11 @@ class Decoder(C.Structure):
                 ("W1", _fp), ("b1", _fp), ("W2", _fp), ("b2", _fp), ("W3", _fp), ("b3", _fp), ("text", _fp)]
 
 
+class MuonTensor(C.Structure):
+    _fields_ = [("weights", _fp), ("grads", _fp), ("momenta", _fp), ("n", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32),
+                ("scale", C.c_double), ("grad_dtype", C.c_int32), ("reserved0", C.c_int32)]
+
+
 _SIGS = {
     "mlpsp_last_error": (C.c_char_p, []),
     "mlpsp_abi_version": (C.c_int, []),
@@ -89,8 +94,8 @@ _SIGS = {
                                          _fp, _fp, _fp, _fp, _fp, _fp, _fp, C.c_int64, _fp, _fp]),
     "mlpsp_orthogonalize_waits": (C.c_int, [C.c_int32, C.c_int32]),
     "mlpsp_orthogonalize": (C.c_int, [_fp, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32] + [C.c_double] * 4 + [_fp, _fp, _fp]),
-    "mlpsp_muon_step": (C.c_int, [_fp, _fp, C.c_int32, _fp, _fp, C.c_int64, C.c_int32, C.c_int32, C.c_double, C.c_double, C.c_int32,
-                                  C.c_double, C.c_double, C.c_int32] + [C.c_double] * 4 + [_fp, _fp]),
+    "mlpsp_muon_step": (C.c_int, [C.POINTER(MuonTensor), C.c_int32, _fp, C.c_double, C.c_double, C.c_int32, C.c_double, C.c_int32]
+                        + [C.c_double] * 4 + [_fp, _fp]),
     "mlpsp_decoder_packed_bytes": (C.c_int64, [C.POINTER(Decoder), C.c_int32]),
     "mlpsp_pack_decoder": (C.c_int, [C.POINTER(Decoder), C.c_int32, _fp, _fp, _fp]),
     "mlpsp_decode_features": (C.c_int, [C.POINTER(Decoder), C.c_int32, _fp, _fp, C.c_int32, C.c_int32, _fp, _fp, _fp, _fp]),

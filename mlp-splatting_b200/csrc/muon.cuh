@@ -28,6 +28,7 @@ struct NsArgs {
   int32_t small, large;      // X is small x large
   int32_t rs, cs;            // X(i, j) lies at i * rs + j * cs
   int32_t steps, nesterov;
+  int32_t follows;           // behind another launch of the same step, with which it shares nothing it writes
   int32_t near, far;         // bits by which a step may multiply singular values within 1/2, within 1/16
   int32_t vec;               // elements of a row that may be moved at once: 1, 2 or 4 (large is a multiple, addresses are aligned)
   float a, b, c, eps;
@@ -139,6 +140,18 @@ __device__ __forceinline__ void ns_split(float x0, float x1, uint32_t& hi, uint3
 __device__ __forceinline__ float2 ns_join(uint32_t hi, uint32_t lo) {
   const float2 h = ns_unpack<false>(hi), l = ns_unpack<false>(lo);
   return make_float2(h.x + l.x, h.y + l.y);
+}
+
+// The launches of one step touch different matrices, so each may start while the one before still runs, whose last tiles (or whose few, for
+// single large matrices) leave most of the GPU idle.  What came before the step is done when any of them starts: the first waits for it
+// before it lets the second be set up, and so on; and since a follower waits for its predecessor before it ends, the last one ends last.
+__device__ __forceinline__ void ns_begin(const NsArgs& q) {
+  if (!q.follows) chain_wait();
+  else __threadfence();
+  chain_release();
+}
+__device__ __forceinline__ void ns_end(const NsArgs& q) {
+  if (q.follows) chain_wait();
 }
 
 // matrices of at most kNsWarpRows x kNsWarpCols go to the warp kernel (muon_warp.cu), others to the cluster kernel (muon_tc.cu)

@@ -12,13 +12,14 @@
 
 namespace mlpsp {
 
-constexpr int kNtThreads = 256, kNtRows = 128, kNtChunk = kNtRows * 16;
+constexpr int kNtThreads = 512, kNtParts = 4;      // four threads per row: the parts of its columns
+constexpr int kNtRows = 128, kNtChunk = kNtRows * 16;
 constexpr int kNtMaxCols = 256, kNtMaxCluster = 8;
 constexpr int kNtTmemCols = 256;
 constexpr uint32_t kNtMnB = 1u << 16;      // bit 16 of the instruction descriptor: B is MN-major
 
 // shared memory: X hi | X lo (NP / 8 chunks each) | A hi | A lo (16 chunks each; the FP32 parts of A pass through here too) | small
-constexpr int kNtSmall = 2 * kNtRows * 16 + 16 + 64;
+constexpr int kNtSmall = kNtParts * kNtRows * 16 + (kNtRows + 1) * 16 + 64;
 __host__ __device__ constexpr int nt_smem(int np) { return np * (2 * kNtChunk / 8) + 32 * kNtChunk + kNtSmall; }
 static_assert(nt_smem(kNtMaxCols) <= 227 * 1024, "a CTA's shared memory");
 
@@ -40,25 +41,47 @@ __device__ __forceinline__ void nt_cluster_sync() {
 }
 __device__ __forceinline__ void nt_fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
+__device__ __forceinline__ void nt_put(char* hi, char* lo, const uint32_t (&h)[8], const uint32_t (&l)[8]) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    *reinterpret_cast<uint4*>(hi + e * kNtChunk) = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+    *reinterpret_cast<uint4*>(lo + e * kNtChunk) = make_uint4(l[4 * e], l[4 * e + 1], l[4 * e + 2], l[4 * e + 3]);
+  }
+}
+__device__ __forceinline__ void nt_get(const char* hi, const char* lo, float (&x)[16]) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint4 h4 = *reinterpret_cast<const uint4*>(hi + e * kNtChunk), l4 = *reinterpret_cast<const uint4*>(lo + e * kNtChunk);
+    const uint32_t h[4] = {h4.x, h4.y, h4.z, h4.w}, l[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = ns_join(h[i], l[i]);
+      x[e * 8 + 2 * i] = v.x;
+      x[e * 8 + 2 * i + 1] = v.y;
+    }
+  }
+}
+
 // `np` columns per CTA, `pack` matrices per tile (1 in a cluster)
 __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const int np, const int cluster, const int pack, const int64_t tiles) {
-  chain_wait();
-  chain_release();
+  ns_begin(q);
   extern __shared__ __align__(1024) char smem[];
   const int tid = threadIdx.x, warp = warp_of_cta();
-  const int row = tid & (kNtRows - 1), half = tid >> 7;          // the tile's row of this thread; which half of the columns
+  const int row = tid & (kNtRows - 1), part = tid >> 7;          // the tile's row of this thread; which part of the columns
   const uint32_t sb = smem_u32(smem);
   const uint32_t xh = sb, xl = sb + np * (kNtChunk / 8), ah = xl + np * (kNtChunk / 8), al = ah + 16 * kNtChunk;
-  char* const pxh = smem;
-  char* const pxl = smem + np * (kNtChunk / 8);
+  char* const pxh = smem + row * 16;                               // this thread's row in the first chunk
+  char* const pxl = pxh + np * (kNtChunk / 8);
   char* const pah = pxl + np * (kNtChunk / 8);
   char* const pal = pah + 16 * kNtChunk;
-  float4* const s_part = reinterpret_cast<float4*>(pal + 16 * kNtChunk);      // [2][128] squares of a row's halves: plain, shrunk, grown
-  // between the norms: [128] the diagonal of bA + cA^2, and [2][128] each the halves' sums of squares of a row of X and of A
-  float* const s_diag = reinterpret_cast<float*>(s_part);
-  float* const s_xsq = s_diag + kNtRows;
-  float* const s_asq = s_xsq + 2 * kNtRows;
-  float4* const s_rank = s_part + 2 * kNtRows;                               // this CTA's sums, read by the cluster's others
+  // [4][128] squares of a row's parts: plain, shrunk, grown | [128] sums of the tile's matrices | this CTA's, read by the cluster's others
+  float4* const s_part = reinterpret_cast<float4*>(smem + np * (2 * kNtChunk / 8) + 32 * kNtChunk);
+  float4* const s_sum = s_part + kNtParts * kNtRows;
+  float4* const s_rank = s_sum + kNtRows;
+  // between the norms: [128] the diagonal of A, and [4][128] each the parts' sums of squares of a row of X and of A
+  float* const s_diag = reinterpret_cast<float*>(s_sum);
+  float* const s_xsq = reinterpret_cast<float*>(s_part);
+  float* const s_asq = s_xsq + kNtParts * kNtRows;
   uint32_t* const s_word = reinterpret_cast<uint32_t*>(s_rank + 1);           // mbarrier (two words) | tensor memory | gave up
   const uint32_t bar = smem_u32(s_word);
   uint32_t rank = 0u;
@@ -76,7 +99,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
   const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
   const uint32_t idesc_a = instr_desc(kNtRows, kNtRows), idesc_x = instr_desc(kNtRows, np) | kNtMnB;
   const int sub = row / q.small, srow = row - sub * q.small;       // matrix of the tile and row in it (sub >= pack: none)
-  const int groups = np / 16;
+  const int groups = np / 16;                                      // of 16 columns; a thread has part, part + 4, ...
   const int col0 = (int)rank * np;
   uint32_t phase = 0u;
   bool ok = true;
@@ -93,158 +116,175 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
     __syncthreads();
     tc_fence_after();
   };
+  // `steps` pairs of operands that lie `da` and `db` bytes apart: lo hi and hi lo products, then hi hi (the tensor core rounds a sum towards
+  // zero with every MMA, so the small ones come first)
+  auto product = [&](uint32_t to, uint64_t a_hi, uint64_t a_lo, uint64_t b_hi, uint64_t b_lo, int steps, int da, int db, uint32_t idesc) {
+    if (warp == 0) {
+      if (elect_one()) {
+        for (int s = 0; s < steps; ++s) {
+          const uint64_t oa = (uint64_t)(s * da >> 4), ob = (uint64_t)(s * db >> 4);
+          mma_f16(to, a_hi + oa, b_lo + ob, idesc, s > 0);
+          mma_f16(to, a_lo + oa, b_hi + ob, idesc, 1u);
+        }
+        for (int s = 0; s < steps; ++s) mma_f16(to, a_hi + (uint64_t)(s * da >> 4), b_hi + (uint64_t)(s * db >> 4), idesc, 1u);
+        mma_commit(bar);
+      }
+      __syncwarp();
+    }
+  };
 
   for (int64_t tile = blockIdx.x / cluster; tile < tiles; tile += gridDim.x / cluster) {
     const int64_t k = tile * pack + sub;
     const bool in = sub < pack && k < q.count && (!q.active || q.active[k]);
     const int64_t base = in ? k * q.stride + (int64_t)srow * q.rs : 0;
     if (!__syncthreads_or(in)) continue;         // the same answer in every CTA of a cluster: it holds one matrix
-    // ---- pass one: momentum, sums of squares.  Each thread has the groups of 16 columns half, half + 2, ... of its row.
+    // ---- momentum, and the update's values in FP32 in the places of X's pairs (eight to a pair of 16-byte words); sums of squares
     float4 ss = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto square = [&](float u) {
-      const float s = u * kNsShrink, g = u * kNsGrow;
-      ss.x = fmaf(u, u, ss.x);
-      ss.y = fmaf(s, s, ss.y);
-      ss.z = fmaf(g, g, ss.z);
-    };
-    auto fetch = [&](int64_t at, auto n, bool first) {
-      constexpr int N = decltype(n)::value;
-      NsVec<N> v = ns_load<N>(q.g, at, q.type);
-      if (q.m) {
-        NsVec<N> m = ns_load<N>(q.m, at, MLPSP_PRECISION_F32);
+    auto load = [&](auto width) {
+      constexpr int N = decltype(width)::value;
+      for (int gr = part; gr < groups; gr += kNtParts) {
+        const int c = col0 + gr * 16;
+        float u[16];
+        NsVec<N> v[16 / N], m[16 / N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          if (first) m.v[e] = ns_new_momentum(q, v.v[e], m.v[e]);
-          v.v[e] = ns_update(q, v.v[e], m.v[e]);
+        for (int i = 0; i < 16 / N; ++i)
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[i].v[e] = m[i].v[e] = 0.f;
+        auto at = [&](int i) { return base + (N == 4 ? (int64_t)(c + N * i) : (int64_t)(c + i) * q.cs); };
+        if (in) {
+#pragma unroll
+          for (int i = 0; i < 16 / N; ++i)
+            if (c + N * i < q.large) {
+              v[i] = ns_load<N>(q.g, at(i), q.type);
+              if (q.m) m[i] = ns_load<N>(q.m, at(i), MLPSP_PRECISION_F32);
+            }
         }
-        if (first) ns_store<N>(q.m, at, MLPSP_PRECISION_F32, m);
-      }
-      return v;
-    };
-    for (int gr = half; gr < groups; gr += 2) {
-      const int c = col0 + gr * 16;
-      if (!in) break;
-      if (q.vec == 4) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          if (c + e < q.large) {
-            const NsVec<4> v = fetch(base + c + e, NsTag<4>{}, true);
+        for (int i = 0; i < 16 / N; ++i) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) square(v.v[i]);
+          for (int e = 0; e < N; ++e) {
+            float x = v[i].v[e];
+            if (q.m) {
+              m[i].v[e] = ns_new_momentum(q, x, m[i].v[e]);
+              x = ns_update(q, x, m[i].v[e]);
+            }
+            u[i * N + e] = x;
+            const float s = x * kNsShrink, g = x * kNsGrow;
+            ss.x = fmaf(x, x, ss.x);
+            ss.y = fmaf(s, s, ss.y);
+            ss.z = fmaf(g, g, ss.z);
           }
-      } else {
-        for (int e = 0; e < 16; ++e)
-          if (c + e < q.large) square(fetch(base + (int64_t)(c + e) * q.cs, NsTag<1>{}, true).v[0]);
+          if (q.m && in && c + N * i < q.large) ns_store<N>(q.m, at(i), MLPSP_PRECISION_F32, m[i]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          *reinterpret_cast<float4*>(pxh + (gr * 2 + e) * kNtChunk) = make_float4(u[8 * e], u[8 * e + 1], u[8 * e + 2], u[8 * e + 3]);
+          *reinterpret_cast<float4*>(pxl + (gr * 2 + e) * kNtChunk) = make_float4(u[8 * e + 4], u[8 * e + 5], u[8 * e + 6], u[8 * e + 7]);
+        }
+      }
+    };
+    if (q.vec == 4) load(NsTag<4>{});
+    else load(NsTag<1>{});
+    s_part[part * kNtRows + row] = ss;
+    __syncthreads();
+    // a warp adds up a matrix, or every sixteenth
+    for (int p = warp; p < pack; p += kNtThreads / 32) {
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int r = p * q.small + (tid & 31); r < (p + 1) * q.small; r += 32)
+#pragma unroll
+        for (int w = 0; w < kNtParts; ++w) {
+          const float4 o = s_part[w * kNtRows + r];
+          sum.x += o.x; sum.y += o.y; sum.z += o.z;
+        }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
+        sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
+        sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o);
+      }
+      if ((tid & 31) == 0) {
+        s_sum[p] = sum;
+        if (p == 0) *s_rank = sum;
       }
     }
-    s_part[half * kNtRows + row] = ss;
-    __syncthreads();
+    if (cluster > 1) nt_cluster_sync();
+    else __syncthreads();
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float4& o) { sum.x += o.x; sum.y += o.y; sum.z += o.z; };
-    if (sub < pack)
-      for (int r = sub * q.small; r < (sub + 1) * q.small; ++r) {
-        add(s_part[r]);
-        add(s_part[kNtRows + r]);
-      }
     if (cluster > 1) {
-      if (tid == 0) *s_rank = sum;
-      nt_cluster_sync();
-      sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int r = 0; r < cluster; ++r) add(nt_peer_load(nt_map(smem_u32(s_rank), r)));
-      nt_cluster_sync();
+      float4 o[kNtMaxCluster];
+#pragma unroll
+      for (int r = 0; r < kNtMaxCluster; ++r)
+        if (r < cluster) o[r] = nt_peer_load(nt_map(smem_u32(s_rank), r));
+#pragma unroll
+      for (int r = 0; r < kNtMaxCluster; ++r)
+        if (r < cluster) { sum.x += o[r].x; sum.y += o[r].y; sum.z += o[r].z; }
+    } else if (sub < pack) {
+      sum = s_sum[sub];
     }
     const bool huge = !(sum.x < __int_as_float(0x7f800000)), tiny = sum.x < kNsTinySquares;
     const NsStart start = ns_start(q.eps, huge ? sum.y : tiny ? sum.z : sum.x, huge ? kNsShrink : tiny ? kNsGrow : 1.f);
     const bool lost = start.lost;
     int k2 = start.k;
-    // ---- pass two: X0 as binary16 pairs
-    __syncthreads();         // the norms' sums have been read
+    // ---- X0 as binary16 pairs, in place
     float xsq = 0.f;
-    for (int gr = half; gr < groups; gr += 2) {
-      const int c = col0 + gr * 16;
-      float u[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) u[e] = 0.f;
-      if (in && !lost) {
-        if (q.vec == 4) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            if (c + e < q.large) {
-              const NsVec<4> v = fetch(base + c + e, NsTag<4>{}, false);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) u[e + i] = v.v[i] * start.pre * start.inv;
-            }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (c + e < q.large) u[e] = fetch(base + (int64_t)(c + e) * q.cs, NsTag<1>{}, false).v[0] * start.pre * start.inv;
-        }
-      }
+    for (int gr = part; gr < groups; gr += kNtParts) {
+      char* const ph = pxh + gr * 2 * kNtChunk;
+      char* const pl = pxl + gr * 2 * kNtChunk;
       uint32_t h[8], l[8];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) xsq = fmaf(u[e], u[e], xsq);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ns_split(u[2 * e], u[2 * e + 1], h[e], l[e]);
-#pragma unroll
       for (int e = 0; e < 2; ++e) {
-        *reinterpret_cast<uint4*>(pxh + (gr * 2 + e) * kNtChunk + row * 16) = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
-        *reinterpret_cast<uint4*>(pxl + (gr * 2 + e) * kNtChunk + row * 16) = make_uint4(l[4 * e], l[4 * e + 1], l[4 * e + 2], l[4 * e + 3]);
+        const float4 a = *reinterpret_cast<const float4*>(ph + e * kNtChunk), b = *reinterpret_cast<const float4*>(pl + e * kNtChunk);
+        const float u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            x[j] = lost ? 0.f : u[2 * i + j] * start.pre * start.inv;
+            xsq = fmaf(x[j], x[j], xsq);
+          }
+          ns_split(x[0], x[1], h[e * 4 + i], l[e * 4 + i]);
+        }
       }
+      nt_put(ph, pl, h, l);
     }
-    s_xsq[half * kNtRows + row] = xsq;
+    __syncthreads();         // the norms' sums have been read
+    s_xsq[part * kNtRows + row] = xsq;
     ready();
     for (int it = 0; it < q.steps; ++it) {
       const NsStep by = ns_step(q, k2);
       // ---- A = X X^T
-      if (warp == 0) {
-        if (elect_one()) {
-          const uint64_t dh = smem_desc(xh, kNtChunk, 128), dl = smem_desc(xl, kNtChunk, 128);
-          // the small products first: the tensor core rounds a sum towards zero with every MMA
-          for (int s = 0; s < groups; ++s) {
-            const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4);
-            mma_f16(tmem, dh + o, dl + o, idesc_a, s > 0);
-            mma_f16(tmem, dl + o, dh + o, idesc_a, 1u);
-          }
-          for (int s = 0; s < groups; ++s) {
-            const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4);
-            mma_f16(tmem, dh + o, dh + o, idesc_a, 1u);
-          }
-          mma_commit(bar);
-        }
-        __syncwarp();
+      {
+        const uint64_t dh = smem_desc(xh, kNtChunk, 128), dl = smem_desc(xl, kNtChunk, 128);
+        product(tmem, dh, dl, dh, dl, groups, 2 * kNtChunk, 2 * kNtChunk, idesc_a);
       }
-      wait();
       // The diagonals of A and A^2, sums of squares of rows, are taken from FP32 sums: the tensor core's, rounded towards zero with every
       // MMA, are all too small by a few 1e-7, and the iteration carries that on (4e-6 of the result for 128 rows)
-      const float xx = s_xsq[row] + s_xsq[kNtRows + row];
-      float asq = 0.f;
+      float xx = 0.f;
+#pragma unroll
+      for (int w = 0; w < kNtParts; ++w) xx += s_xsq[w * kNtRows + row];
+      wait();
       if (cluster == 1) {
-        for (int gr = half; gr < 8; gr += 2) {
+        for (int gr = part; gr < 8; gr += kNtParts) {
           uint32_t d[16], h[8], l[8];
           tmem_ld16(trow + gr * 16, d);
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (gr * 16 + e == row) d[e] = __float_as_uint(xx);
+          const int off = gr * 16 - row;       // column less row
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             float v[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const int c = gr * 16 + 2 * e + i;
-              v[i] = (unsigned)(c - sub * q.small) < (unsigned)q.small ? __uint_as_float(d[2 * e + i]) * by.gram : 0.f;
+              const int c = 2 * e + i;
+              v[i] = (off + c == 0 ? xx : __uint_as_float(d[c])) * by.gram;
+              if ((unsigned)(off + c + srow) >= (unsigned)q.small) v[i] = 0.f;
             }
-            asq = fmaf(v[0], v[0], fmaf(v[1], v[1], asq));
             ns_split(v[0], v[1], h[e], l[e]);
           }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            *reinterpret_cast<uint4*>(pah + (gr * 2 + e) * kNtChunk + row * 16) = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
-            *reinterpret_cast<uint4*>(pal + (gr * 2 + e) * kNtChunk + row * 16) = make_uint4(l[4 * e], l[4 * e + 1], l[4 * e + 2], l[4 * e + 3]);
-          }
+          nt_put(pah + gr * 2 * kNtChunk, pal + gr * 2 * kNtChunk, h, l);
         }
       } else {
         // the slices' parts of A: 32 pieces of [128 rows][4 columns] in FP32, each added up by one CTA and handed to all
-        for (int gr = half; gr < 8; gr += 2) {
+        for (int gr = part; gr < 8; gr += kNtParts) {
           uint32_t d[16];
           tmem_ld16(trow + gr * 16, d);
 #pragma unroll
@@ -252,177 +292,146 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
             if (gr * 16 + e == row) d[e] = __float_as_uint(xx);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(pah + (gr * 4 + e) * kNtChunk + row * 16) = make_uint4(d[4 * e], d[4 * e + 1], d[4 * e + 2], d[4 * e + 3]);
+            *reinterpret_cast<uint4*>(pah + (gr * 4 + e) * kNtChunk) = make_uint4(d[4 * e], d[4 * e + 1], d[4 * e + 2], d[4 * e + 3]);
         }
         nt_cluster_sync();
-        float4 t[8];
-        // unit u = (piece, row): of the 16 rounds of 256 units this CTA takes rank, rank + cluster, ...
+        constexpr int kRounds = 32 * kNtRows / kNtThreads;       // of the units (piece, row); this CTA takes rank, rank + cluster, ...
+        float4 t[kRounds / 2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kRounds / 2; ++j) {
           const int round = j * cluster + (int)rank;
           t[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (round < 16) {
+          if (round < kRounds) {
             const uint32_t at = ah + (uint32_t)(round * kNtThreads + tid) * 16;
-            for (int r = 0; r < cluster; ++r) {
-              const float4 o = nt_peer_load(nt_map(at, r));
-              t[j].x += o.x; t[j].y += o.y; t[j].z += o.z; t[j].w += o.w;
-            }
+            float4 o[kNtMaxCluster];
+#pragma unroll
+            for (int r = 0; r < kNtMaxCluster; ++r)
+              if (r < cluster) o[r] = nt_peer_load(nt_map(at, r));
+#pragma unroll
+            for (int r = 0; r < kNtMaxCluster; ++r)
+              if (r < cluster) { t[j].x += o[r].x; t[j].y += o[r].y; t[j].z += o[r].z; t[j].w += o[r].w; }
           }
         }
         nt_cluster_sync();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kRounds / 2; ++j) {
           const int round = j * cluster + (int)rank;
-          if (round < 16) {
+          if (round < kRounds) {
             const int u = round * kNtThreads + tid, piece = u >> 7, r0 = u & (kNtRows - 1);
             uint32_t h[2], l[2];
             ns_split(t[j].x * by.gram, t[j].y * by.gram, h[0], l[0]);
             ns_split(t[j].z * by.gram, t[j].w * by.gram, h[1], l[1]);
             const uint32_t at = (uint32_t)((piece >> 1) * kNtChunk + r0 * 16 + (piece & 1) * 8);
-            for (int r = 0; r < cluster; ++r) {
-              nt_peer_store2(nt_map(ah + at, r), h[0], h[1]);
-              nt_peer_store2(nt_map(al + at, r), l[0], l[1]);
-            }
+#pragma unroll
+            for (int r = 0; r < kNtMaxCluster; ++r)
+              if (r < cluster) {
+                nt_peer_store2(nt_map(ah + at, r), h[0], h[1]);
+                nt_peer_store2(nt_map(al + at, r), l[0], l[1]);
+              }
           }
         }
         nt_fence_async();
         nt_cluster_sync();
-        for (int gr = half; gr < 8; gr += 2)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint4 h4 = *reinterpret_cast<const uint4*>(pah + (gr * 2 + e) * kNtChunk + row * 16);
-            const uint4 l4 = *reinterpret_cast<const uint4*>(pal + (gr * 2 + e) * kNtChunk + row * 16);
-            const uint32_t h[4] = {h4.x, h4.y, h4.z, h4.w}, l[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { const float2 a = ns_join(h[i], l[i]); asq = fmaf(a.x, a.x, fmaf(a.y, a.y, asq)); }
-          }
       }
-      s_asq[half * kNtRows + row] = asq;
       ready();
       // ---- A^2
-      if (warp == 0) {
-        if (elect_one()) {
-          const uint64_t dh = smem_desc(ah, kNtChunk, 128), dl = smem_desc(al, kNtChunk, 128);
-          for (int s = 0; s < 8; ++s) {
-            const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4);
-            mma_f16(tmem + kNtRows, dh + o, dl + o, idesc_a, s > 0);
-            mma_f16(tmem + kNtRows, dl + o, dh + o, idesc_a, 1u);
-          }
-          for (int s = 0; s < 8; ++s) {
-            const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4);
-            mma_f16(tmem + kNtRows, dh + o, dh + o, idesc_a, 1u);
-          }
-          mma_commit(bar);
-        }
-        __syncwarp();
+      {
+        const uint64_t dh = smem_desc(ah, kNtChunk, 128), dl = smem_desc(al, kNtChunk, 128);
+        product(tmem + kNtRows, dh, dl, dh, dl, 8, 2 * kNtChunk, 2 * kNtChunk, idesc_a);
       }
       wait();
-      const float aa = s_asq[row] + s_asq[kNtRows + row];
-      for (int gr = half; gr < 8; gr += 2) {
-        uint32_t d[16];
+      // ---- P = b A + c A^2 but for its diagonal, which is kept apart (muon_warp.cu)
+      float asq = 0.f;
+      for (int gr = part; gr < 8; gr += kNtParts) {
+        uint32_t d[16], h[8], l[8];
+        float a[16];
         tmem_ld16(trow + kNtRows + gr * 16, d);
+        nt_get(pah + gr * 2 * kNtChunk, pal + gr * 2 * kNtChunk, a);
+        const int off = row - gr * 16;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (gr * 16 + e == row) d[e] = __float_as_uint(aa);
+        for (int e = 0; e < 8; ++e) {
+          float p[2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint4* const sh = reinterpret_cast<uint4*>(pah + (gr * 2 + e) * kNtChunk + row * 16);
-          uint4* const sl = reinterpret_cast<uint4*>(pal + (gr * 2 + e) * kNtChunk + row * 16);
-          const uint4 h4 = *sh, l4 = *sl;
-          uint32_t h[4] = {h4.x, h4.y, h4.z, h4.w}, l[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 a = ns_join(h[i], l[i]);
-            float p0 = fmaf(by.b, a.x, by.c * __uint_as_float(d[e * 8 + 2 * i])), p1 = fmaf(by.b, a.y, by.c * __uint_as_float(d[e * 8 + 2 * i + 1]));
-            const int c = gr * 16 + e * 8 + 2 * i;
-            if (c == (row & ~1)) {       // the diagonal is kept apart (muon_warp.cu)
-              s_diag[row] = row & 1 ? p1 : p0;
-              if (row & 1) p1 = 0.f; else p0 = 0.f;
-            }
-            ns_split(p0, p1, h[i], l[i]);
+          for (int i = 0; i < 2; ++i) {
+            const int c = 2 * e + i;
+            asq = fmaf(a[c], a[c], asq);
+            p[i] = fmaf(by.b, a[c], by.c * __uint_as_float(d[c]));
+            if (off == c) { s_diag[row] = a[c]; p[i] = 0.f; }
           }
-          *sh = make_uint4(h[0], h[1], h[2], h[3]);
-          *sl = make_uint4(l[0], l[1], l[2], l[3]);
+          ns_split(p[0], p[1], h[e], l[e]);
         }
+        nt_put(pah + gr * 2 * kNtChunk, pal + gr * 2 * kNtChunk, h, l);
       }
+      s_asq[part * kNtRows + row] = asq;
       ready();
-      // ---- (bA + cA^2) X, over the accumulators that have been read
-      if (warp == 0) {
-        if (elect_one()) {
-          const uint64_t ph = smem_desc(ah, kNtChunk, 128), pl = smem_desc(al, kNtChunk, 128);
-          const uint64_t dh = smem_desc(xh, 128, kNtChunk), dl = smem_desc(xl, 128, kNtChunk);
-          for (int s = 0; s < 8; ++s) {
-            const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4), n = (uint64_t)(s * 256 >> 4);
-            mma_f16(tmem, ph + o, dl + n, idesc_x, s > 0);
-            mma_f16(tmem, pl + o, dh + n, idesc_x, 1u);
-          }
-          for (int s = 0; s < 8; ++s) {
-            const uint64_t o = (uint64_t)(s * 2 * kNtChunk >> 4), n = (uint64_t)(s * 256 >> 4);
-            mma_f16(tmem, ph + o, dh + n, idesc_x, 1u);
-          }
-          mma_commit(bar);
-        }
-        __syncwarp();
-      }
-      wait();
+      // ---- P X, over the accumulators that have been read
+      product(tmem, smem_desc(ah, kNtChunk, 128), smem_desc(al, kNtChunk, 128), smem_desc(xh, 128, kNtChunk), smem_desc(xl, 128, kNtChunk), 8,
+              2 * kNtChunk, 256, idesc_x);
       const bool last = it + 1 == q.steps;
-      const float own = by.a + s_diag[row];
+      float own = by.b * s_diag[row] + by.a;
+#pragma unroll
+      for (int w = 0; w < kNtParts; ++w) own = fmaf(by.c, s_asq[w * kNtRows + row], own);
       xsq = 0.f;
-      if (last && !ok) atomicOr(s_word + 3, 1u);
-      if (last) __syncthreads();
+      wait();
+      if (last) {
+        if (!ok) atomicOr(s_word + 3, 1u);
+        __syncthreads();
+      }
       const bool write = last && in && s_word[3] == 0u;
-      for (int gr = half; gr < groups; gr += 2) {
-        uint32_t d[16];
-        tmem_ld16(trow + gr * 16, d);
+      for (int gr = part; gr < groups; gr += kNtParts) {
+        char* const ph = pxh + gr * 2 * kNtChunk;
+        char* const pl = pxl + gr * 2 * kNtChunk;
+        uint32_t d[16], h[8], l[8];
         float v[16];
+        const int c = col0 + gr * 16;
+        NsVec<4> w[4];
+        const bool stepping = write && q.m && q.vec == 4;
+        if (stepping) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint4* const sh = reinterpret_cast<uint4*>(pxh + (gr * 2 + e) * kNtChunk + row * 16);
-          uint4* const sl = reinterpret_cast<uint4*>(pxl + (gr * 2 + e) * kNtChunk + row * 16);
-          const uint4 h4 = *sh, l4 = *sl;
-          uint32_t h[4] = {h4.x, h4.y, h4.z, h4.w}, l[4] = {l4.x, l4.y, l4.z, l4.w};
+          for (int e = 0; e < 4; ++e)
+            if (c + 4 * e < q.large) w[e] = ns_load<4>(q.w, base + c + 4 * e, MLPSP_PRECISION_F32);
+        }
+        tmem_ld16(trow + gr * 16, d);
+        nt_get(ph, pl, v);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 x = ns_join(h[i], l[i]);
-            v[e * 8 + 2 * i] = fmaf(own, x.x, __uint_as_float(d[e * 8 + 2 * i]));
-            v[e * 8 + 2 * i + 1] = fmaf(own, x.y, __uint_as_float(d[e * 8 + 2 * i + 1]));
-            xsq = fmaf(v[e * 8 + 2 * i], v[e * 8 + 2 * i], fmaf(v[e * 8 + 2 * i + 1], v[e * 8 + 2 * i + 1], xsq));
-            ns_split(v[e * 8 + 2 * i], v[e * 8 + 2 * i + 1], h[i], l[i]);
+        for (int e = 0; e < 16; ++e) v[e] = fmaf(own, v[e], __uint_as_float(d[e]));
+        if (!last) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            xsq = fmaf(v[2 * e], v[2 * e], fmaf(v[2 * e + 1], v[2 * e + 1], xsq));
+            ns_split(v[2 * e], v[2 * e + 1], h[e], l[e]);
           }
-          if (!last) {
-            *sh = make_uint4(h[0], h[1], h[2], h[3]);
-            *sl = make_uint4(l[0], l[1], l[2], l[3]);
-          }
+          nt_put(ph, pl, h, l);
         }
         if (!write) continue;
-        const int c = col0 + gr * 16;
-        const float nan = __int_as_float(0x7fffffff), fin = ns_exp2i(-10 - k2);
+        const float fin = lost ? __int_as_float(0x7fffffff) : ns_exp2i(-10 - k2);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] *= fin;
         if (q.vec == 4) {
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            if (c + e < q.large) {
+          for (int e = 0; e < 4; ++e)
+            if (c + 4 * e < q.large) {
               NsVec<4> r;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) r.v[i] = lost ? nan : v[e + i] * fin;
-              if (q.m) {
-                const NsVec<4> w = ns_load<4>(q.w, base + c + e, MLPSP_PRECISION_F32);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) r.v[i] = fmaf(-q.step, r.v[i], q.keep * w.v[i]);
-                ns_store<4>(q.w, base + c + e, MLPSP_PRECISION_F32, r);
-              } else ns_store<4>(q.out, base + c + e, q.type, r);
+              for (int i = 0; i < 4; ++i) r.v[i] = q.m ? fmaf(-q.step, v[4 * e + i], q.keep * w[e].v[i]) : v[4 * e + i];
+              if (q.m) ns_store<4>(q.w, base + c + 4 * e, MLPSP_PRECISION_F32, r);
+              else ns_store<4>(q.out, base + c + 4 * e, q.type, r);
             }
         } else {
+          float u[16];
+          if (q.m)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = c + e < q.large ? q.w[base + (int64_t)(c + e) * q.cs] : 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (c + e < q.large) {
               const int64_t at = base + (int64_t)(c + e) * q.cs;
-              const float r = lost ? nan : v[e] * fin;
-              if (q.m) q.w[at] = fmaf(-q.step, r, q.keep * q.w[at]);
-              else ns_store<1>(q.out, at, q.type, NsVec<1>{{r}});
+              if (q.m) q.w[at] = fmaf(-q.step, v[e], q.keep * u[e]);
+              else ns_store<1>(q.out, at, q.type, NsVec<1>{{v[e]}});
             }
         }
       }
-      s_xsq[half * kNtRows + row] = xsq;
+      s_xsq[part * kNtRows + row] = xsq;
       ready();
     }
   }
@@ -430,6 +439,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
   __syncthreads();
   if (warp == 0) tmem_free(tmem, kNtTmemCols);
   if (cluster > 1) nt_cluster_sync();      // no CTA leaves while another may read its shared memory
+  ns_end(q);
 }
 
 int launch_ns_cluster(const NsArgs& q, cudaStream_t st) {
@@ -441,8 +451,7 @@ int launch_ns_cluster(const NsArgs& q, cudaStream_t st) {
   const int smem = nt_smem(np);
   static DeviceOnce once;
   if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, nt_smem(kNtMaxCols)));
-  const int resident = std::max(1, std::min(2, 227 * 1024 / (smem + 1024)));
-  const int64_t most = std::max<int64_t>(1, (int64_t)sm_count() * resident / cluster);
+  const int64_t most = std::max<int64_t>(1, (int64_t)sm_count() / cluster);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(std::min(tiles, most) * cluster));
   cfg.blockDim = dim3(kNtThreads);
@@ -483,7 +492,7 @@ static bool ns_bounded(double a, double b, double c, int steps) {
 
 // what the two entries share
 static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a, double b, double c,
-                     double eps, cudaStream_t st) {
+                     double eps, cudaStream_t st, bool launch = true) {
   MLPSP_REQUIRE(n >= 0 && rows >= 1 && cols >= 1, MLPSP_E_ARG, "%s: bad sizes", who);
   MLPSP_REQUIRE(std::min(rows, cols) <= MLPSP_MUON_MAX_SMALL && std::max(rows, cols) <= MLPSP_MUON_MAX_LARGE, MLPSP_E_LIMIT,
                 "%s: %d x %d matrices; at most %d on the smaller and %d on the larger side", who, rows, cols, MLPSP_MUON_MAX_SMALL,
@@ -495,6 +504,7 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
   MLPSP_REQUIRE(ns_bounded(a, b, c, steps), MLPSP_E_ARG, "%s: singular values leave [0, 4] with these coefficients", who);
   if (n == 0) return MLPSP_OK;
   MLPSP_REQUIRE(q.g && (q.m ? q.w != nullptr : q.out != nullptr), MLPSP_E_ARG, "%s: null pointer", who);
+  if (!launch) return MLPSP_OK;
   const bool tall = rows > cols;
   q.count = n;
   q.stride = (int64_t)rows * cols;
@@ -535,24 +545,36 @@ extern "C" int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n,
   return ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream);
 }
 
-extern "C" int mlpsp_muon_step(float* weights, const void* grads, int32_t grad_dtype, float* momenta, const uint8_t* active, int64_t n,
-                               int32_t rows, int32_t cols, double lr, double momentum, int32_t nesterov, double weight_decay, double scale,
-                               int32_t steps, double a, double b, double c, double eps, int32_t* status, void* stream) {
-  MLPSP_REQUIRE(n <= 0 || (weights && grads && momenta), MLPSP_E_ARG, "mlpsp_muon_step: null pointer");
+extern "C" int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, const uint8_t* active, double lr, double momentum,
+                               int32_t nesterov, double weight_decay, int32_t steps, double a, double b, double c, double eps,
+                               int32_t* status, void* stream) {
+  MLPSP_REQUIRE(count >= 0 && (count == 0 || tensors), MLPSP_E_ARG, "mlpsp_muon_step: null pointer");
   MLPSP_REQUIRE(momentum >= 0.0 && momentum < 1.0, MLPSP_E_ARG, "mlpsp_muon_step: momentum must be within [0, 1)");
-  MLPSP_REQUIRE(lr >= 0.0 && lr < 1e30 && weight_decay >= 0.0 && weight_decay < 1e30 && scale > 0.0 && scale < 1e30, MLPSP_E_ARG,
-                "mlpsp_muon_step: lr, weight_decay and scale must be finite and not negative");
-  NsArgs q = {};
-  q.g = grads;
-  q.m = momenta;
-  q.w = weights;
-  q.active = active;
-  q.type = grad_dtype;
-  q.status = status;
-  q.nesterov = nesterov != 0;
-  q.momentum = (float)momentum;
-  q.rest = (float)(1.0 - momentum);
-  q.keep = (float)(1.0 - lr * weight_decay);
-  q.step = (float)(lr * scale);
-  return ns_launch("mlpsp_muon_step", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream);
+  MLPSP_REQUIRE(lr >= 0.0 && lr < 1e30 && weight_decay >= 0.0 && weight_decay < 1e30, MLPSP_E_ARG,
+                "mlpsp_muon_step: lr and weight_decay must be finite and not negative");
+  for (int pass = 0; pass < 2; ++pass) {       // all tensors are checked before the first launch
+    bool follows = false;
+    for (int32_t i = 0; i < count; ++i) {
+      const mlpsp_muon_tensor& t = tensors[i];
+      MLPSP_REQUIRE(t.n <= 0 || (t.weights && t.grads && t.momenta), MLPSP_E_ARG, "mlpsp_muon_step: null pointer");
+      MLPSP_REQUIRE(t.scale > 0.0 && t.scale < 1e30, MLPSP_E_ARG, "mlpsp_muon_step: scale must be finite and positive");
+      NsArgs q = {};
+      q.g = t.grads;
+      q.m = t.momenta;
+      q.w = t.weights;
+      q.active = active;
+      q.type = t.grad_dtype;
+      q.status = status;
+      q.nesterov = nesterov != 0;
+      q.momentum = (float)momentum;
+      q.rest = (float)(1.0 - momentum);
+      q.keep = (float)(1.0 - lr * weight_decay);
+      q.step = (float)(lr * t.scale);
+      q.follows = follows;
+      const int rc = ns_launch("mlpsp_muon_step", q, t.n, t.rows, t.cols, steps, a, b, c, eps, (cudaStream_t)stream, pass == 1);
+      if (rc) return rc;
+      follows |= t.n > 0;
+    }
+  }
+  return MLPSP_OK;
 }

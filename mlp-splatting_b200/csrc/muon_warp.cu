@@ -118,8 +118,7 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
   constexpr int KH = MB == 1 ? 2 : 1;       // with one block of rows, rows h = 0 and 1 of a lane may belong to two matrices
   constexpr int kPanels = (NB + 1) / 2, kPanel = ns_panel_bytes<MB>(), kLo = kPanel / 2, kBlock = 16 * 32;
   extern __shared__ __align__(128) char smem[];
-  chain_wait();
-  chain_release();
+  ns_begin(q);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   char* const mine = smem + (threadIdx.x >> 5) * ns_warp_smem<MB, NB>();
   const uint32_t xs = smem_u32(mine);
@@ -551,6 +550,7 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
       __syncwarp();
     }
   }
+  ns_end(q);
 }
 
 template <int MB, int NB, int CTAS>

@@ -114,9 +114,6 @@ def muon_step(weights, grads, momenta, *, lr: float, momentum: float = 0.95, nes
         if g.shape != w.shape or m.shape != w.shape:
             raise ValueError("a weight, its gradient and its momentum must have one shape")
     dev = _check_tensors([t for k in lists for t in k] + ([] if active is None else [active]))
-    written = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for k in (lists[0], lists[2]) for t in k if t.numel())
-    if any(a[1] > b[0] for a, b in zip(written, written[1:])):
-        raise ValueError("weights and momenta must not overlap")
     if active is not None and (active.dtype != torch.bool or active.ndim != 1
                                or any(w.ndim != 3 or w.shape[0] != active.numel() for w in lists[0])):
         raise ValueError("active must be bool [N], and every weight a stack of N matrices")
@@ -124,11 +121,19 @@ def muon_step(weights, grads, momenta, *, lr: float, momentum: float = 0.95, nes
     lr, momentum, weight_decay = float(lr), float(momentum), float(weight_decay)
     if not (0.0 <= lr < 1e30 and 0.0 <= weight_decay < 1e30 and 0.0 <= momentum < 1.0):
         raise ValueError("lr and weight_decay must be finite and not negative, momentum within [0, 1)")
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), k != 1) for k in range(3) for t in lists[k] if t.numel())
+    reached = [0, 0]        # where the arrays so far end: any of them, written ones
+    for first, end, written in spans:
+        if first < reached[0 if written else 1]:
+            raise ValueError("weights and momenta must not overlap each other or a gradient")
+        reached[0] = max(reached[0], end)
+        reached[1] = max(reached[1], end if written else 0)
     lib = L.load()
     with _on(dev):
         status, st = _status(dev, shapes, check), _stream_ptr(dev)
-        for w, g, m, (n, rows, cols) in zip(*lists, shapes):
-            L.check(lib.mlpsp_muon_step(L.ptr(w), L.ptr(g), _TYPES[g.dtype], L.ptr(m), L.ptr(active), n, rows, cols, lr, momentum,
-                                        int(bool(nesterov)), weight_decay, math.sqrt(max(1.0, rows / cols)), *args, L.ptr(status), st),
-                    "mlpsp_muon_step")
+        tensors = (L.MuonTensor * len(shapes))(*(
+            (L.ptr(w), L.ptr(g), L.ptr(m), n, rows, cols, math.sqrt(max(1.0, rows / cols)), _TYPES[g.dtype], 0)
+            for w, g, m, (n, rows, cols) in zip(*lists, shapes)))
+        L.check(lib.mlpsp_muon_step(tensors, len(shapes), L.ptr(active), lr, momentum, int(bool(nesterov)), weight_decay, *args,
+                                    L.ptr(status), st), "mlpsp_muon_step")
         _read_status(status, "muon_step")

@@ -24,9 +24,14 @@ def test_c_entries_check_their_arguments():
     assert ortho(update=None) == -1 and ortho(out=None) == -1 and b"null pointer" in lib.mlpsp_last_error()
     assert ortho(n=0, update=None, out=None) == 0      # nothing to do: no launch
 
-    def step(w=FAKE, g=FAKE, m=FAKE, lr=0.1, mu=0.9, wd=0.0, scale=1.0):
-        return lib.mlpsp_muon_step(w, g, 0, m, None, 1, 32, 72, lr, mu, 1, wd, scale, *NS, None, None)
+    def step(w=FAKE, g=FAKE, m=FAKE, lr=0.1, mu=0.9, wd=0.0, scale=1.0, rows=32):
+        good = L.MuonTensor(None, None, None, 0, 32, 72, 1.0, 0, 0)      # nothing in it
+        tensors = (L.MuonTensor * 2)(good, L.MuonTensor(w, g, m, 1, rows, 72, scale, 0, 0))
+        return lib.mlpsp_muon_step(tensors, 2, None, lr, mu, 1, wd, *NS, None, None)
 
+    assert step(rows=0) == -1
+    assert lib.mlpsp_muon_step(None, 1, None, 0.1, 0.9, 1, 0.0, *NS, None, None) == -1
+    assert lib.mlpsp_muon_step(None, 0, None, 0.1, 0.9, 1, 0.0, *NS, None, None) == 0
     assert step(w=None) == -1 and step(g=None) == -1 and step(m=None) == -1
     assert step(mu=1.0) == -1 and step(mu=-0.1) == -1 and step(lr=-1.0) == -1 and step(lr=float("inf")) == -1
     assert step(wd=float("nan")) == -1 and step(scale=0.0) == -1

@@ -33,14 +33,9 @@ __device__ __forceinline__ float4 nt_peer_load(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void nt_peer_store2(uint32_t addr, uint32_t a, uint32_t b) {
-  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
-}
 __device__ __forceinline__ void nt_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void nt_fence_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
-
 __device__ __forceinline__ void nt_put(char* hi, char* lo, const uint32_t (&h)[8], const uint32_t (&l)[8]) {
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -295,43 +290,41 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
             *reinterpret_cast<uint4*>(pah + (gr * 4 + e) * kNtChunk) = make_uint4(d[4 * e], d[4 * e + 1], d[4 * e + 2], d[4 * e + 3]);
         }
         nt_cluster_sync();
-        constexpr int kRounds = 32 * kNtRows / kNtThreads;       // of the units (piece, row); this CTA takes rank, rank + cluster, ...
-        float4 t[kRounds / 2];
+        // this thread: row `row` of piece `part` of the groups that fall to this CTA, in place (no other reads them here)
+        for (int gr = (int)rank; gr < 8; gr += cluster) {
+          const uint32_t at = ah + (uint32_t)((gr * 4 + part) * kNtChunk + row * 16);
+          float4 o[kNtMaxCluster];
 #pragma unroll
-        for (int j = 0; j < kRounds / 2; ++j) {
-          const int round = j * cluster + (int)rank;
-          t[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (round < kRounds) {
-            const uint32_t at = ah + (uint32_t)(round * kNtThreads + tid) * 16;
-            float4 o[kNtMaxCluster];
+          for (int r = 0; r < kNtMaxCluster; ++r)
+            if (r < cluster) o[r] = nt_peer_load(nt_map(at, r));
+          float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int r = 0; r < kNtMaxCluster; ++r)
-              if (r < cluster) o[r] = nt_peer_load(nt_map(at, r));
+          for (int r = 0; r < kNtMaxCluster; ++r)
+            if (r < cluster) { t.x += o[r].x; t.y += o[r].y; t.z += o[r].z; t.w += o[r].w; }
+          *reinterpret_cast<float4*>(pah + (gr * 4 + part) * kNtChunk) = t;
+        }
+        nt_cluster_sync();
+        // ... and everyone fetches the sums from their owners.  (Handing them out with remote stores took 12 of 24 us an iteration.)
+        float4 t[2][4];
 #pragma unroll
-            for (int r = 0; r < kNtMaxCluster; ++r)
-              if (r < cluster) { t[j].x += o[r].x; t[j].y += o[r].y; t[j].z += o[r].z; t[j].w += o[r].w; }
-          }
+        for (int j = 0; j < 2; ++j) {
+          const int gr = part + j * kNtParts;
+          const uint32_t at = nt_map(ah + (uint32_t)(gr * 4 * kNtChunk + row * 16), (uint32_t)(gr % cluster));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[j][e] = nt_peer_load(at + e * kNtChunk);
         }
         nt_cluster_sync();
 #pragma unroll
-        for (int j = 0; j < kRounds / 2; ++j) {
-          const int round = j * cluster + (int)rank;
-          if (round < kRounds) {
-            const int u = round * kNtThreads + tid, piece = u >> 7, r0 = u & (kNtRows - 1);
-            uint32_t h[2], l[2];
-            ns_split(t[j].x * by.gram, t[j].y * by.gram, h[0], l[0]);
-            ns_split(t[j].z * by.gram, t[j].w * by.gram, h[1], l[1]);
-            const uint32_t at = (uint32_t)((piece >> 1) * kNtChunk + r0 * 16 + (piece & 1) * 8);
+        for (int j = 0; j < 2; ++j) {
+          const int gr = part + j * kNtParts;
+          uint32_t h[8], l[8];
 #pragma unroll
-            for (int r = 0; r < kNtMaxCluster; ++r)
-              if (r < cluster) {
-                nt_peer_store2(nt_map(ah + at, r), h[0], h[1]);
-                nt_peer_store2(nt_map(al + at, r), l[0], l[1]);
-              }
+          for (int e = 0; e < 4; ++e) {
+            ns_split(t[j][e].x * by.gram, t[j][e].y * by.gram, h[2 * e], l[2 * e]);
+            ns_split(t[j][e].z * by.gram, t[j][e].w * by.gram, h[2 * e + 1], l[2 * e + 1]);
           }
+          nt_put(pah + gr * 2 * kNtChunk, pal + gr * 2 * kNtChunk, h, l);
         }
-        nt_fence_async();
-        nt_cluster_sync();
       }
       ready();
       // ---- A^2

@@ -110,11 +110,14 @@ __device__ __forceinline__ void ns_prefetch(const void* p, int64_t i, int n, int
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const char*>(p) + i * size), "r"(n * size) : "memory");
 }
 
-// prefetch: whole tiles may be brought into L2 ahead of their use.  A warp's own loads and products follow each other, and the warps of an SM
-// fall into step (all load, then all multiply); with the next tile's gradient and momentum and this one's weights on their way meanwhile,
-// loading is short: 100,000 steps of 32 x 72 matrices 2,001 -> 1,660 us.
+// One tile per warp: which tiles an SM takes is left to the hardware.  With as many CTAs as fit the GPU walking the tiles in turn, the
+// slowest SM set the time and its warps fell into step, all loading and then all multiplying: a step of 100,000 matrices of 32 x 72
+// 2,540 us, now 1,720 (of which 704 are its bytes).  prefetch: a tile's weights, wanted last, are brought into L2 when it starts (1,817
+// without).  Twenty warps per SM instead of sixteen: 2,160.
+constexpr int kNsWarps = 1;       // per CTA: places fall free one by one
+
 template <int MB, int NB, int CTAS>
-__global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int pack, const int64_t tiles, const bool prefetch) {
+__global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(const NsArgs q, const int pack, const int64_t tiles, const bool prefetch) {
   constexpr int KH = MB == 1 ? 2 : 1;       // with one block of rows, rows h = 0 and 1 of a lane may belong to two matrices
   constexpr int kPanels = (NB + 1) / 2, kPanel = ns_panel_bytes<MB>(), kLo = kPanel / 2, kBlock = 16 * 32;
   extern __shared__ __align__(128) char smem[];
@@ -141,7 +144,9 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
 #pragma unroll
         for (int e = 0; e < 2; ++e) same |= (sub[h] == (n * 8 + 2 * t + e) / q.small ? 1u : 0u) << (h * 4 + n * 2 + e);
   }
-  for (int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); tile < tiles; tile += (int64_t)gridDim.x * 4) {
+  const int64_t tile = (int64_t)blockIdx.x * kNsWarps + (threadIdx.x >> 5);
+  auto work = [&] {
+    if (tile >= tiles) return;
     // element of the first column of this lane's rows; rows of block mb and half h are `in`
     int64_t first[KH];
     bool on[KH];
@@ -151,15 +156,10 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
       on[h] = sub[h] >= 0 && k < q.count && (!q.active || q.active[k]);
       first[h] = on[h] ? k * q.stride + (int64_t)row[h] * q.rs : 0;
     }
-    if (!__any_sync(0xffffffffu, on[0] || on[KH - 1])) continue;
-    if (prefetch && lane == 0) {
-      const int n = pack * (int)q.stride, size = q.type == MLPSP_PRECISION_F32 ? 4 : 2;
-      const int64_t next = tile + (int64_t)gridDim.x * 4;
-      if (q.m && (tile + 1) * pack <= q.count) ns_prefetch(q.w, tile * n, n, 4);
-      if ((next + 1) * pack <= q.count && (!q.active || pack > 1 || q.active[next])) {
-        ns_prefetch(q.g, next * n, n, size);
-        if (q.m) ns_prefetch(q.m, next * n, n, 4);
-      }
+    if (!__any_sync(0xffffffffu, on[0] || on[KH - 1])) return;
+    if (prefetch && lane == 0 && q.m && (tile + 1) * pack <= q.count) {
+      const int n = pack * (int)q.stride;
+      ns_prefetch(q.w, tile * n, n, 4);
     }
     auto in = [&](int mb, int h) { return on[h % KH] && (MB == 1 || mb * 16 + h * 8 + g < q.small); };
     auto base = [&](int mb, int h) { return MB == 1 ? first[h % KH] : first[0] + (int64_t)((mb * 16 + h * 8) * q.rs); };
@@ -547,31 +547,31 @@ __global__ void __launch_bounds__(128, CTAS) k_ns_warp(const NsArgs q, const int
 #pragma unroll 1
       for (int p = 0; p < NB / 2; ++p) finish(p, NsTag<2>{});
       if (NB & 1) finish(NB / 2, NsTag<1>{});
-      __syncwarp();
     }
-  }
+  };
+  work();
   ns_end(q);
 }
 
 template <int MB, int NB, int CTAS>
 static int ns_warp(const NsArgs& q, cudaStream_t st) {
-  constexpr int smem = 4 * ns_warp_smem<MB, NB>();
-  static_assert(CTAS * (smem + 1024) <= 227 * 1024, "resident CTAs");
+  constexpr int smem = kNsWarps * ns_warp_smem<MB, NB>();
+  static_assert(CTAS * 4 / kNsWarps * (smem + 1024) <= 227 * 1024, "resident CTAs");
   static DeviceOnce once;
   if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_warp<MB, NB, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const int pack = std::max(1, 16 * MB / q.small);
-  const int64_t tiles = (q.count + pack - 1) / pack;
-  const unsigned grid = (unsigned)std::min<int64_t>((tiles + 3) / 4, (int64_t)sm_count() * CTAS);
-  const uintptr_t all = reinterpret_cast<uintptr_t>(q.g) | reinterpret_cast<uintptr_t>(q.m) | reinterpret_cast<uintptr_t>(q.w);
-  const bool prefetch = all % 16 == 0 && pack * q.stride * (q.type == MLPSP_PRECISION_F32 ? 4 : 2) % 16 == 0;
+  const int64_t tiles = (q.count + pack - 1) / pack, grid = (tiles + kNsWarps - 1) / kNsWarps;
+  MLPSP_REQUIRE(grid < (1ll << 31), MLPSP_E_LIMIT, "orthogonalize: too many matrices");
+  const bool prefetch = reinterpret_cast<uintptr_t>(q.w) % 16 == 0 && pack * q.stride % 4 == 0;
   LaunchScope scope(kKMisc, 1, st);
-  return cuda_check(launch_chained(k_ns_warp<MB, NB, CTAS>, dim3(grid), dim3(128), smem, st, q, pack, tiles, prefetch), "orthogonalize");
+  return cuda_check(launch_chained(k_ns_warp<MB, NB, CTAS>, dim3((unsigned)grid), dim3(32 * kNsWarps), smem, st, q, pack, tiles, prefetch),
+                    "orthogonalize");
 }
 
 int launch_ns_warp(const NsArgs& q, cudaStream_t st) {
   const int nb = (q.large + 7) / 8;
   if (q.small <= 16) return nb <= 4 ? ns_warp<1, 4, 8>(q, st) : nb <= 6 ? ns_warp<1, 6, 7>(q, st) : nb <= 9 ? ns_warp<1, 9, 7>(q, st) : ns_warp<1, 12, 7>(q, st);
-  return nb <= 4 ? ns_warp<2, 4, 4>(q, st) : nb <= 6 ? ns_warp<2, 6, 4>(q, st) : nb <= 9 ? ns_warp<2, 9, 3>(q, st) : ns_warp<2, 12, 4>(q, st);
+  return nb <= 4 ? ns_warp<2, 4, 4>(q, st) : nb <= 6 ? ns_warp<2, 6, 4>(q, st) : nb <= 9 ? ns_warp<2, 9, 4>(q, st) : ns_warp<2, 12, 4>(q, st);
 }
 
 }  // namespace mlpsp

@@ -330,14 +330,13 @@ int mlpsp_group_rows(const int32_t* primitive_ids, int64_t num_records, int32_t 
 
 /* The place of every record among the records grouped by primitive (stable: records of one primitive keep their order):
  * offsets[n+1] int64 as mlpsp_group_records writes them, slots[R] int32 with 0 <= slots[r] < R, a permutation.  An id outside
- * [0, n) drops its record: it takes a place at offsets[n] or behind.  R < 2^31; scratch as mlpsp_group_records. */
-int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_records, int32_t n, int64_t* offsets, int32_t* slots,
-                        void* scratch, int64_t scratch_bytes, void* stream);
-
-/* *findings_host (HOST) receives MLPSP_ROUTE_BAD_OFFSETS when pixel_offsets[pixels+1] does not start at zero, end at records
- * or ascend, else 0; the call waits for the answer. */
+ * [0, n) drops its record: it takes a place at offsets[n] or behind.  R < 2^31.
+ * findings_host (HOST, or NULL) receives MLPSP_ROUTE_BAD_OFFSETS when pixel_offsets[pixels+1] does not start at zero, end at R
+ * or ascend, else 0; the call then waits for the answer, not for the places. */
 #define MLPSP_ROUTE_BAD_OFFSETS 1
-int mlpsp_check_pixel_offsets(const int64_t* pixel_offsets, int64_t pixels, int64_t records, int32_t* findings_host, void* stream);
+int64_t mlpsp_route_records_scratch_bytes(int64_t num_records, int32_t n);
+int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_records, int32_t n, const int64_t* pixel_offsets, int64_t pixels,
+                        int64_t* offsets, int32_t* slots, void* scratch, int64_t scratch_bytes, int32_t* findings_host, void* stream);
 
 /* In the three calls below the records of pixel p are fan * p .. fan * (p + 1) - 1 (pixel_offsets NULL, records = pixels * fan)
  * or pixel_offsets[p] .. pixel_offsets[p + 1] - 1 (int64 [pixels + 1], from zero to records, ascending); slots and kept =

@@ -123,8 +123,8 @@ _SIGS = {
     "mlpsp_group_records_scratch_bytes": (C.c_int64, [C.c_int64, C.c_int32]),
     "mlpsp_group_records": (C.c_int, [_fp, C.c_int64, C.c_int32, _fp, _fp, _fp, C.c_int64, _fp]),
     "mlpsp_group_rows": (C.c_int, [_fp, C.c_int64, C.c_int32, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, C.c_int64, _fp]),
-    "mlpsp_route_records": (C.c_int, [_fp, C.c_int64, C.c_int32, _fp, _fp, _fp, C.c_int64, _fp]),
-    "mlpsp_check_pixel_offsets": (C.c_int, [_fp, C.c_int64, C.c_int64, C.POINTER(C.c_int32), _fp]),
+    "mlpsp_route_records_scratch_bytes": (C.c_int64, [C.c_int64, C.c_int32]),
+    "mlpsp_route_records": (C.c_int, [_fp, C.c_int64, C.c_int32, _fp, C.c_int64, _fp, _fp, _fp, C.c_int64, _fp, _fp]),
     "mlpsp_dispatch_rows": (C.c_int, [_fp, C.c_int32, C.c_int64, C.c_int64, C.c_int32, _fp, _fp, C.c_int64, _fp, _fp, _fp]),
     "mlpsp_combine_rows": (C.c_int, [_fp, C.c_int32, C.c_int64, _fp, C.c_int64, C.c_int32, _fp, _fp, C.c_int64, _fp, _fp, _fp]),
     "mlpsp_combine_rows_gradients": (C.c_int, [_fp, _fp, C.c_int32, C.c_int64, _fp, C.c_int64, C.c_int32, _fp, _fp, C.c_int64, _fp,

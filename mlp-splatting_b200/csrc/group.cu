@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kGsThreads) k_gs_scan(int nblocks, int32_t* __
   if (threadIdx.x == 0) dtot[blockIdx.x] = run;
 }
 
-// LAST: order and inverse (each where given) instead of vals_out
+// LAST: order and inverse (where given) instead of vals_out
 template <bool FIRST, bool LAST>
 __global__ void __launch_bounds__(kGsThreads) k_gs_scatter(
     const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int64_t n, int nprim, int shift, int dbits, int nblocks,
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kGsThreads) k_gs_scatter(
       keys_out[dst] = it.x;
       if (!LAST) vals_out[dst] = it.y;
       else {
-        if (order) order[dst] = (int64_t)it.y;
+        order[dst] = (int64_t)it.y;
         if (inverse) inverse[it.y] = (uint32_t)dst;
       }
     }
@@ -229,13 +229,12 @@ static GsLayout gs_layout(int64_t R) {
   return L;
 }
 
-// slots (where given) receives the place of every record
 static int group_rows(const int32_t* ids, int64_t R, int n, int64_t* offsets, int64_t* order, const float* x6, const float* d4,
                       const int32_t* masks, float* x6_out, float* d4_out, int32_t* masks_out, void* scratch,
-                      int64_t scratch_bytes, cudaStream_t st, const char* who, int32_t* slots = nullptr) {
+                      int64_t scratch_bytes, cudaStream_t st, const char* who) {
   MLPSP_REQUIRE(R >= 0 && n >= 0 && offsets, MLPSP_E_ARG, "%s: bad arguments", who);
   MLPSP_REQUIRE(R < (1ll << 31), MLPSP_E_LIMIT, "%s: more than 2^31-1 records", who);
-  MLPSP_REQUIRE(R == 0 || (ids && (order || slots)), MLPSP_E_ARG, "%s: null pointer", who);
+  MLPSP_REQUIRE(R == 0 || (ids && order), MLPSP_E_ARG, "%s: null pointer", who);
   MLPSP_REQUIRE((!x6 || x6_out) && (!d4 || d4_out) && (!masks || masks_out), MLPSP_E_ARG, "%s: null pointer", who);
   const GsLayout L = gs_layout(R);
   MLPSP_REQUIRE(scratch && scratch_bytes >= L.bytes, MLPSP_E_SCRATCH, "%s: scratch needs %lld bytes", who, (long long)L.bytes);
@@ -253,8 +252,7 @@ static int group_rows(const int32_t* ids, int64_t R, int n, int64_t* offsets, in
     const bool first = pass == 0, last = pass == g.passes - 1;
     uint32_t* k_out = (uint32_t*)(b + L.key[pass & 1]);
     uint32_t* v_out = (uint32_t*)(b + L.val[pass & 1]);          // the last pass writes no values: their place takes the inverse
-    if (last && slots) inverse = reinterpret_cast<uint32_t*>(slots);
-    else if (last && (x6 || d4 || masks)) inverse = v_out;
+    if (last && (x6 || d4 || masks)) inverse = v_out;
     launch_chained(first ? k_gs_hist<true> : k_gs_hist<false>, dim3(g.nblocks), dim3(kGsThreads), 0, st, k_in, R, n, shift, g.dbits, g.nblocks, hist);
     launch_chained(k_gs_scan, dim3(1 << g.dbits), dim3(kGsThreads), 0, st, g.nblocks, hist, dtot);
     auto* scatter = first ? (last ? k_gs_scatter<true, true> : k_gs_scatter<true, false>) : (last ? k_gs_scatter<false, true> : k_gs_scatter<false, false>);
@@ -263,7 +261,6 @@ static int group_rows(const int32_t* ids, int64_t R, int n, int64_t* offsets, in
     k_in = k_out;
     v_in = v_out;
   }
-  if (slots) inverse = nullptr;        // no rows to move: the last kernel writes the offsets only
   const int64_t span = std::max<int64_t>(inverse ? R : 0, (int64_t)n + 1);
   launch_chained(k_gs_finish, dim3((unsigned)((span + 255) / 256)), dim3(256), 0, st, k_in, inverse, R, n, offsets,
                  reinterpret_cast<const float2*>(x6), reinterpret_cast<const float4*>(d4), reinterpret_cast<const int2*>(masks),
@@ -296,12 +293,6 @@ extern "C" int mlpsp_group_rows(const int32_t* primitive_ids, int64_t num_record
                 MLPSP_E_ARG, "mlpsp_group_rows: x6 and masks must be 8-byte aligned, grad4 16-byte aligned");
   return group_rows(primitive_ids, num_records, n, offsets, order, x6, grad4, relu_masks, x6_out, grad4_out, masks_out, scratch,
                     scratch_bytes, (cudaStream_t)stream, "mlpsp_group_rows");
-}
-
-extern "C" int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_records, int32_t n, int64_t* offsets, int32_t* slots,
-                                   void* scratch, int64_t scratch_bytes, void* stream) {
-  return group_rows(primitive_ids, num_records, n, offsets, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, scratch,
-                    scratch_bytes, (cudaStream_t)stream, "mlpsp_route_records", slots);
 }
 
 extern "C" int mlpsp_prepare_groups(const int64_t* offsets, int32_t n, int64_t segment_size, int64_t* group_offsets,

@@ -174,20 +174,6 @@ __global__ void __launch_bounds__(kRtThreads) k_combine_grad(const typename RtPi
   }
 }
 
-// bit 0: the pixel offsets do not start at zero, end at the record count or ascend
-__global__ void k_route_check(const int64_t* __restrict__ offsets, int64_t pixels, int64_t records, volatile int32_t* __restrict__ found) {
-  chain_wait();
-  chain_release();
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-  bool bad = false;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i <= pixels; i += stride) {
-    const int64_t o = __ldg(offsets + i);
-    bad |= i == 0 ? o != 0 : o < __ldg(offsets + i - 1);
-    bad |= i == pixels && o != records;
-  }
-  if (bad) *found = MLPSP_ROUTE_BAD_OFFSETS;
-}
-
 // the widest piece that divides the row and all addresses
 static int rt_piece(int64_t row_bytes, std::initializer_list<const void*> ptrs) {
   uintptr_t all = (uintptr_t)row_bytes;
@@ -258,25 +244,6 @@ using namespace mlpsp;
   if (dtype == MLPSP_PRECISION_F32) {                                                                             \
     if (piece == 16) call(float, 16); else if (piece == 8) call(float, 8); else call(float, 4);                   \
   } else if (dtype == MLPSP_PRECISION_F16) { MLPSP_BY_PIECE(__half, call) } else { MLPSP_BY_PIECE(__nv_bfloat16, call) }
-
-extern "C" int mlpsp_check_pixel_offsets(const int64_t* pixel_offsets, int64_t pixels, int64_t records, int32_t* findings_host,
-                                         void* stream) {
-  MLPSP_REQUIRE(pixel_offsets && findings_host && pixels >= 0 && records >= 0, MLPSP_E_ARG, "mlpsp_check_pixel_offsets: bad arguments");
-  cudaStream_t st = (cudaStream_t)stream;
-  HostWords& hw = host_words();
-  cudaEvent_t ev = nullptr;
-  const int rc = hw.open(&ev);
-  if (rc) return rc;
-  hw.word[0] = 0;
-  LaunchScope scope(kKMisc, 1, st);
-  launch_chained(k_route_check, dim3((unsigned)std::min<int64_t>(sm_count() * 8, pixels / 1024 + 1)), dim3(256), 0, st, pixel_offsets, pixels,
-                 records, static_cast<volatile int32_t*>(hw.word));
-  MLPSP_CUDA_OK(cudaGetLastError());
-  MLPSP_CUDA_OK(cudaEventRecord(ev, st));
-  MLPSP_CUDA_OK(cudaEventSynchronize(ev));
-  *findings_host = *static_cast<volatile int32_t*>(hw.word);
-  return MLPSP_OK;
-}
 
 extern "C" int mlpsp_dispatch_rows(const void* x, int32_t dtype, int64_t dim, int64_t pixels, int32_t fan, const int64_t* pixel_offsets,
                                    const int32_t* slots, int64_t records, const int64_t* kept, void* out, void* stream) {

@@ -198,17 +198,14 @@ def route_records(primitive_ids: torch.Tensor, num_primitives: int, pixel_offset
         raise RuntimeError("route_records waits for the check of pixel_offsets: pass check=False inside a graph capture")
     offsets = torch.empty(n + 1, device=dev, dtype=torch.int64)
     slots = torch.empty(R, device=dev, dtype=torch.int32)
-    nbytes = int(lib.mlpsp_group_records_scratch_bytes(R, n))
+    nbytes = int(lib.mlpsp_route_records_scratch_bytes(R, n))
     scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     found = C.c_int32(0)
     with _on(dev):
-        st = _stream_ptr(dev)
-        if first is not None and check:
-            L.check(lib.mlpsp_check_pixel_offsets(L.ptr(first), pixels, R, C.byref(found), st), "mlpsp_check_pixel_offsets")
-            if found.value & L.ROUTE_BAD_OFFSETS:
-                raise ValueError("pixel offsets must start at zero, end at the record count and be monotone")
-        L.check(lib.mlpsp_route_records(L.ptr(ids), R, n, L.ptr(offsets), L.ptr(slots), L.ptr(scratch), nbytes, st),
-                "mlpsp_route_records")
+        L.check(lib.mlpsp_route_records(L.ptr(ids), R, n, L.ptr(first), pixels, L.ptr(offsets), L.ptr(slots), L.ptr(scratch), nbytes,
+                                        C.byref(found) if first is not None and check else None, _stream_ptr(dev)), "mlpsp_route_records")
+    if found.value & L.ROUTE_BAD_OFFSETS:
+        raise ValueError("pixel offsets must start at zero, end at the record count and be monotone")
     return RecordRoute(offsets, slots, pixels, fan, first)
 
 

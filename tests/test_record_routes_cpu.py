@@ -23,10 +23,14 @@ def test_c_entries_check_their_arguments():
     assert b"null pointer" in lib.mlpsp_last_error()
     assert lib.mlpsp_combine_rows_gradients(FAKE, FAKE, 0, 4, None, 2, 2, None, FAKE, 4, FAKE, None, None, None) == -1
     assert lib.mlpsp_combine_rows_gradients(FAKE, None, 0, 4, None, 2, 2, None, FAKE, 4, FAKE, FAKE, FAKE, None) == -1
-    assert lib.mlpsp_route_records(FAKE, 1 << 31, 4, FAKE, FAKE, FAKE, 1 << 40, None) == -4
-    assert lib.mlpsp_route_records(FAKE, 4, 4, FAKE, None, FAKE, 1 << 20, None) == -1
-    assert lib.mlpsp_route_records(FAKE, 4, 4, FAKE, FAKE, FAKE, 8, None) == -2
-    assert lib.mlpsp_check_pixel_offsets(None, 1, 1, ctypes.byref(ctypes.c_int32()), None) == -1
+    def route(ids=FAKE, R=4, n=4, offsets=FAKE, slots=FAKE, nbytes=1 << 20, found=None):
+        return lib.mlpsp_route_records(ids, R, n, None, 0, offsets, slots, FAKE, nbytes, found, None)
+
+    assert route(R=1 << 31, nbytes=1 << 40) == -4 and route(n=2 ** 31 - 1) == -4 and route(R=-1) == -1
+    assert route(slots=None) == -1 and route(ids=None) == -1 and route(offsets=None) == -1
+    assert route(nbytes=8) == -2 and b"scratch needs" in lib.mlpsp_last_error()
+    assert route(found=ctypes.byref(ctypes.c_int32())) == -1 and b"no pixel offsets" in lib.mlpsp_last_error()
+    assert lib.mlpsp_route_records_scratch_bytes(-1, 3) == -1 and lib.mlpsp_route_records_scratch_bytes(1000, 70_000) > 12_000
     # nothing to do: no launch, no pointer is looked at
     assert lib.mlpsp_dispatch_rows(None, 0, 4, 0, 2, None, None, 0, FAKE, None, None) == 0
 

@@ -1,12 +1,13 @@
 // The places of records among the records grouped by primitive: slots[r], a stable counting sort that moves no rows and whose result is the
 // inverse of the usual permutation.
 //
-// Least significant digit first, nine bits a pass: one pass for up to 510 primitives, two up to 262,142 (mlpsp_group_records takes digits of
+// Least significant digit first, nine bits a pass: one pass for up to 511 primitives, two up to 262,143 (mlpsp_group_records takes digits of
 // at most eight, evenly split).  A CTA owns 4,096 records in a row, a warp 256 of them.  Per pass: counts of every digit and CTA; their
 // exclusive prefix over the CTAs, a CTA per digit; and the placement, in which a warp ranks its records with match.any against its own
 // counters.  Passes before the last reorder (key, record) in shared memory and write runs.  The last one only needs each record's place:
 // it is written straight from registers (to slots[record]: in order if there was one pass, else scattered), and the sorted keys behind it
 // when there is more than one digit, for the offsets, which are found by binary search inside the range of their highest digit.
+// Up to 65,536 records of up to 511 primitives take one launch of a cluster of eight CTAs.
 //
 // Bound: latency of the ranking (sixteen warps a CTA, three CTAs per SM; the same passes at two CTAs of eight took 95 us each for
 // 7.3 M records) and, in the last pass of several, the scattered words.  7.3 M records of 100,000 primitives: 330 -> 148 us; 32,764 of
@@ -81,10 +82,33 @@ __global__ void __launch_bounds__(kRsThreads) k_rs_scan(int nblocks, int32_t* __
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
+// ranks of a warp's records, round by round, among those of the same digit before them; cnt: the warp's counters, zero at first.
+// left: records from this lane's first on (a record every 32).
+template <int ROUNDS>
+__device__ __forceinline__ void rs_rank(const uint32_t (&key)[ROUNDS], int64_t left, int rounds, int shift, uint32_t mask, uint16_t* cnt, uint32_t lt,
+                                        int (&rank)[ROUNDS]) {
+  uint32_t peers[ROUNDS];      // all of them before the counters' chain begins
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if (r < rounds) peers[r] = __match_any_sync(0xffffffffu, r * 32 < left ? (key[r] >> shift) & mask : 0x1000u);
+  __syncwarp();
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if (r < rounds) {
+      const bool valid = r * 32 < left;
+      const uint32_t d = (key[r] >> shift) & mask;
+      const int before = valid ? cnt[d] : 0;
+      rank[r] = before + __popc(peers[r] & lt);
+      __syncwarp();
+      if (valid && (peers[r] & lt) == 0u) cnt[d] = (uint16_t)(before + __popc(peers[r]));
+      __syncwarp();
+    }
+}
+
 // FIRST: the values are the positions.  LAST: slots[value] = place, instead of values in their places; offsets (only where a digit is the
 // whole key): the first places of all digits, by block 0.
 template <bool FIRST, bool LAST>
-__global__ void __launch_bounds__(kRsThreads, 2) k_rs_place(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int64_t n, int nprim,
+__global__ void __launch_bounds__(kRsThreads, 3) k_rs_place(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ vals, int64_t n, int nprim,
                                                             int shift, uint32_t mask, int nblocks, const int32_t* __restrict__ counts,
                                                             const int32_t* __restrict__ totals, uint32_t* __restrict__ keys_out,
                                                             uint32_t* __restrict__ vals_out, int32_t* __restrict__ slots,
@@ -103,23 +127,13 @@ __global__ void __launch_bounds__(kRsThreads, 2) k_rs_place(const uint32_t* __re
   int rank[kRsRounds];
 #pragma unroll
   for (int r = 0; r < kRsRounds; ++r) key[r] = base + r * 32 < n ? rs_key<FIRST>(__ldg(keys + base + r * 32), nprim) : 0xffffffffu;
-  __syncwarp();
-#pragma unroll
-  for (int r = 0; r < kRsRounds; ++r) {
-    const bool valid = base + r * 32 < n;
-    const uint32_t d = valid ? (key[r] >> shift) & mask : 0x1000u;
-    const uint32_t peers = __match_any_sync(0xffffffffu, d);
-    const int before = valid ? s_cnt[warp][d] : 0;
-    rank[r] = before + __popc(peers & lt);
-    __syncwarp();
-    if (valid && (peers & lt) == 0u) s_cnt[warp][d] = (uint16_t)(before + __popc(peers));
-    __syncwarp();
-  }
-  __syncthreads();
-  // thread = digit: the warps' first positions inside the digit, the digit's first position in the block and its first place of all
+  // of this thread's digit, on their way while the records are ranked
   const bool live = (uint32_t)tid <= mask;
   const int total_of = live ? __ldg(totals + tid) : 0;
   const int before_us = live ? __ldg(counts + (size_t)tid * nblocks + blockIdx.x) : 0;
+  rs_rank<kRsRounds>(key, n - base, kRsRounds, shift, mask, s_cnt[warp], lt, rank);
+  __syncthreads();
+  // thread = digit: the warps' first positions inside the digit, the digit's first position in the block and its first place of all
   int mine = 0;
 #pragma unroll
   for (int w = 0; w < kRsWarps; ++w) { const int c = s_cnt[w][tid]; s_cnt[w][tid] = (uint16_t)mine; mine += c; }
@@ -167,6 +181,57 @@ __global__ void __launch_bounds__(kRsThreads, 2) k_rs_place(const uint32_t* __re
       vals_out[dst] = it.y;
     }
   }
+}
+
+// The whole of it for few records and primitives in one launch of one cluster: the CTAs' counts pass through distributed shared memory.
+constexpr int kRsClusterCtas = 8, kRsClusterRounds = 16;
+constexpr int64_t kRsClusterRecords = (int64_t)kRsClusterCtas * kRsThreads * kRsClusterRounds;
+__global__ void __cluster_dims__(kRsClusterCtas, 1, 1) __launch_bounds__(kRsThreads) k_rs_cluster(const uint32_t* __restrict__ ids, int n, int nprim,
+                                                                                              int rounds, int32_t* __restrict__ slots,
+                                                                                              int64_t* __restrict__ offsets) {
+  chain_wait();
+  chain_release();
+  __shared__ uint16_t s_cnt[kRsWarps][kRsBins];
+  __shared__ int s_total[kRsBins];
+  __shared__ int s_dst[kRsBins];
+  __shared__ int warp_sums[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank_of = blockIdx.x;
+  const int base = (rank_of * kRsWarps + warp) * rounds * 32 + lane;
+  for (int i = lane; i < kRsBins / 2; i += 32) reinterpret_cast<uint32_t*>(s_cnt[warp])[i] = 0u;
+  uint32_t key[kRsClusterRounds];
+  int rank[kRsClusterRounds];
+#pragma unroll
+  for (int r = 0; r < kRsClusterRounds; ++r)
+    if (r < rounds) key[r] = base + r * 32 < n ? rs_key<true>(__ldg(ids + base + r * 32), nprim) : 0xffffffffu;
+  rs_rank<kRsClusterRounds>(key, n - base, rounds, 0, kRsBins - 1, s_cnt[warp], (1u << lane) - 1u, rank);
+  __syncthreads();
+  int mine = 0;
+#pragma unroll
+  for (int w = 0; w < kRsWarps; ++w) { const int c = s_cnt[w][tid]; s_cnt[w][tid] = (uint16_t)mine; mine += c; }
+  s_total[tid] = mine;
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(s_total + tid);
+  int others[kRsClusterCtas], all = 0, before_us = 0, unused;
+#pragma unroll
+  for (int c = 0; c < kRsClusterCtas; ++c) {
+    uint32_t peer;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(c));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(others[c]) : "r"(peer) : "memory");
+  }
+#pragma unroll
+  for (int c = 0; c < kRsClusterCtas; ++c) {
+    all += others[c];
+    if (c < rank_of) before_us += others[c];
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this CTA has read what it wanted of the others
+  const int global = block_exclusive_scan(all, warp_sums, unused);
+  s_dst[tid] = global + before_us;
+  if (rank_of == 0 && tid <= nprim) offsets[tid] = global;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kRsClusterRounds; ++r)
+    if (r < rounds && base + r * 32 < n) slots[base + r * 32] = s_dst[key[r]] + s_cnt[warp][key[r]] + rank[r];
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");        // no CTA leaves while another may read its counts
 }
 
 // first position of every primitive in the sorted keys; starts: the first positions of the highest digits
@@ -258,6 +323,12 @@ extern "C" int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_rec
   }
   if (R == 0) {
     MLPSP_CUDA_OK(cudaMemsetAsync(offsets, 0, 8 * ((size_t)n + 1), st));
+  } else if (n < kRsBins && R <= kRsClusterRecords) {
+    LaunchScope scope(kKMisc, 1, st);
+    constexpr int per_round = kRsClusterCtas * kRsThreads;
+    launch_chained(k_rs_cluster, dim3(kRsClusterCtas), dim3(kRsThreads), 0, st, reinterpret_cast<const uint32_t*>(primitive_ids), (int)R, n,
+                   (int)((R + per_round - 1) / per_round), slots, offsets);
+    MLPSP_CUDA_OK(cudaGetLastError());
   } else {
     const RsPlan p = rs_plan(R, n);
     LaunchScope scope(kKMisc, 3 * p.passes + (p.passes > 1), st);

@@ -266,3 +266,12 @@ def test_wrong_routes_stay_inside_their_tensors():
     pc.combine_rows_gradients(torch.ones(3, 2, device="cuda"), y, route, torch.ones(6, device="cuda"))
     torch.cuda.synchronize()
     assert bool((guard == 7.0).all())
+
+
+@pytest.mark.parametrize("N", [1, 2, 510, 511, 512, 600, 262_143, 262_144])
+@pytest.mark.parametrize("R", [1, 31, 4096, 4097, 65_536, 65_537, 300_001])
+def test_route_at_the_borders_of_its_passes(N, R):
+    ids = torch.randint(-1, N + 1, (R, 1), generator=torch.Generator().manual_seed(N + R))
+    route = pc.route_records(ids.to(torch.int32).cuda(), N)
+    offsets, slots = plain_route(ids, N)
+    assert torch.equal(route.offsets.cpu(), offsets) and torch.equal(route.slots.cpu().long(), slots)

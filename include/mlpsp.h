@@ -332,7 +332,8 @@ int mlpsp_group_rows(const int32_t* primitive_ids, int64_t num_records, int32_t 
  * offsets[n+1] int64 as mlpsp_group_records writes them, slots[R] int32 with 0 <= slots[r] < R, a permutation.  An id outside
  * [0, n) drops its record: it takes a place at offsets[n] or behind.  R < 2^31.
  * findings_host (HOST, or NULL) receives MLPSP_ROUTE_BAD_OFFSETS when pixel_offsets[pixels+1] does not start at zero, end at R
- * or ascend, else 0; the call then waits for the answer, not for the places. */
+ * or ascend, else 0; the call then waits for the answer, not for the places.  Where no scratch bytes are asked for, scratch may be
+ * NULL. */
 #define MLPSP_ROUTE_BAD_OFFSETS 1
 int64_t mlpsp_route_records_scratch_bytes(int64_t num_records, int32_t n);
 int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_records, int32_t n, const int64_t* pixel_offsets, int64_t pixels,

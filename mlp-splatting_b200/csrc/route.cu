@@ -128,48 +128,93 @@ __global__ void __launch_bounds__(kRtThreads) k_combine(const typename RtPiece<B
   out[(size_t)p * pieces + c] = o;
 }
 
-// `lanes` (a power of two) neighbouring threads take a pixel, so that <dout, y> is reduced by shuffles
-template <typename T, int B>
+// Every record for itself: `lanes` (a power of two) neighbouring threads take one, U records a time whose rows are then on their way together.
+// A block has the records of `ppb` pixels, so slots, weights and dw are read and written in order; the pixel of a record is found by binary
+// search among the block's offsets.  4.6 M records of 16-byte rows: 121 us with a thread per pixel (its dw words lie in 32 sectors), 69 so.
+// U is four for rows that fill a group of eight lanes or more (950,000 rows of 128 bytes 90 us, by twos 98; of 66 bytes in 2-byte pieces 152
+// and 188), else two (16-byte rows 69 us, by fours 77; 16,000 rows of 4,096 bytes, several rounds of a warp, 35 and 45).
+constexpr int kRtPixels = 256;
+template <typename T, int B, int U>
 __global__ void __launch_bounds__(kRtThreads) k_combine_grad(const typename RtPiece<B>::type* __restrict__ dout,
                                                              const typename RtPiece<B>::type* __restrict__ y,
-                                                             const float* __restrict__ weights, RouteView v, int pieces, int lanes,
+                                                             const float* __restrict__ weights, RouteView v, int pieces, int lanes, int ppb,
                                                              typename RtPiece<B>::type* __restrict__ dy, float* __restrict__ dw) {
   chain_wait();
   chain_release();
   using V = typename RtPiece<B>::type;
   constexpr int E = B / (int)sizeof(T);
-  const int sub = threadIdx.x & (lanes - 1);
-  const int64_t p = ((int64_t)blockIdx.x * kRtThreads + threadIdx.x) / lanes;
-  int64_t b = 0, e = 0;
-  if (p < v.pixels) rt_range(v, p, b, e);
+  __shared__ int s_first[kRtPixels + 1];
+  const int64_t p0 = (int64_t)blockIdx.x * ppb;
+  const int here = (int)min((int64_t)ppb, v.pixels - p0);
+  int64_t first = p0 * v.fan, last = (p0 + here) * v.fan;
+  if (v.pixel_offsets) {
+    for (int i = threadIdx.x; i <= here; i += kRtThreads) s_first[i] = (int)min(max(__ldg(v.pixel_offsets + p0 + i), (int64_t)0), v.records);
+    __syncthreads();
+    first = s_first[0];
+    last = s_first[here];
+  }
   const uint32_t kept = rt_kept(v), all = (uint32_t)v.records;
+  const int sub = threadIdx.x & (lanes - 1), groups = kRtThreads / lanes;
   const uint32_t group = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
-  for (int64_t r = b; r < e; ++r) {
-    const uint32_t s = (uint32_t)__ldg(v.slots + r);
-    const float w = weights ? __ldg(weights + r) : 1.f;
-    const bool live = s < kept;
-    float dot = 0.f;
-    for (int c = sub; c < pieces; c += lanes) {
-      const V g = __ldg(dout + (size_t)p * pieces + c);
-      const T* gf = reinterpret_cast<const T*>(&g);
-      if (dw && live) {
-        const V row = __ldg(y + (size_t)s * pieces + c);
-        const T* f = reinterpret_cast<const T*>(&row);
+  for (int64_t r0 = first + threadIdx.x / lanes; r0 < last; r0 += (int64_t)groups * U) {
+    uint32_t s[U];
+    float w[U], dot[U];
+    size_t pixel[U];
 #pragma unroll
-        for (int i = 0; i < E; ++i) dot = fmaf(rt_float(gf[i]), rt_float(f[i]), dot);
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + u * groups;
+      const bool valid = r < last;
+      s[u] = valid ? (uint32_t)__ldg(v.slots + r) : 0xffffffffu;
+      w[u] = valid && weights ? __ldg(weights + r) : 1.f;
+      dot[u] = 0.f;
+      int lo = 0;
+      if (v.pixel_offsets) {       // the last of the block's pixels whose first record is not behind r
+        int hi = here;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (s_first[mid] <= r) lo = mid; else hi = mid;
+        }
+      } else if (valid) {
+        lo = (int)(r - first) / v.fan;
       }
-      if (dy && s < all) {
-        V o = {};
-        T* of = reinterpret_cast<T*>(&o);
-        if (live)
+      pixel[u] = (size_t)(p0 + lo);
+    }
+    for (int c = sub; c < pieces; c += lanes) {
+      V g[U], row[U];
 #pragma unroll
-          for (int i = 0; i < E; ++i) of[i] = rt_round<T>(w * rt_float(gf[i]));
-        dy[(size_t)s * pieces + c] = o;
+      for (int u = 0; u < U; ++u) {
+        if (s[u] < kept) {
+          g[u] = __ldg(dout + pixel[u] * pieces + c);
+          if (dw) row[u] = __ldg(y + (size_t)s[u] * pieces + c);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool live = s[u] < kept;
+        const T* gf = reinterpret_cast<const T*>(&g[u]);
+        if (dw && live) {
+          const T* f = reinterpret_cast<const T*>(&row[u]);
+#pragma unroll
+          for (int i = 0; i < E; ++i) dot[u] = fmaf(rt_float(gf[i]), rt_float(f[i]), dot[u]);
+        }
+        if (dy && s[u] < all) {
+          V o = {};
+          T* of = reinterpret_cast<T*>(&o);
+          if (live)
+#pragma unroll
+            for (int i = 0; i < E; ++i) of[i] = rt_round<T>(w[u] * rt_float(gf[i]));
+          dy[(size_t)s[u] * pieces + c] = o;
+        }
       }
     }
     if (dw) {
-      for (int o = lanes >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(group, dot, o);
-      if (sub == 0) dw[r] = dot;
+      for (int o = lanes >> 1; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) dot[u] += __shfl_xor_sync(group, dot[u], o);
+      if (sub == 0)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (r0 + u * groups < last) dw[r0 + u * groups] = dot[u];
     }
   }
 }
@@ -224,9 +269,9 @@ static void combine_grad(const void* dout, const void* y, const float* weights, 
   const int pieces = (int)(row_bytes / B);
   int lanes = 1;
   while (lanes < 32 && lanes < pieces) lanes *= 2;
-  const int64_t per_block = kRtThreads / lanes;
-  launch_chained(k_combine_grad<T, B>, dim3((unsigned)((v.pixels + per_block - 1) / per_block)), dim3(kRtThreads), 0, st,
-                 static_cast<const V*>(dout), static_cast<const V*>(y), weights, v, pieces, lanes, static_cast<V*>(dy), dw);
+  const int ppb = (int)std::min<int64_t>(kRtPixels, std::max<int64_t>(1, v.pixels / (sm_count() * 8)));      // eight blocks per SM, if pixels last
+  launch_chained(pieces >= 8 && pieces <= 64 ? k_combine_grad<T, B, 4> : k_combine_grad<T, B, 2>, dim3((unsigned)((v.pixels + ppb - 1) / ppb)), dim3(kRtThreads), 0, st, static_cast<const V*>(dout),
+                 static_cast<const V*>(y), weights, v, pieces, lanes, ppb, static_cast<V*>(dy), dw);
 }
 
 }  // namespace mlpsp

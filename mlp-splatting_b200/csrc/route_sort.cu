@@ -276,9 +276,11 @@ static RsPlan rs_plan(int64_t R, int n) {
 }
 // scratch: digit totals | first places | block counts | keys and values of the passes before the last, keys of the last
 struct RsLayout { int64_t totals, starts, counts, key[2], val[2], bytes; };
+static bool rs_in_a_cluster(int64_t R, int n) { return n < kRsBins && R <= kRsClusterRecords; }
 static RsLayout rs_layout(int64_t R, int n) {
   const RsPlan p = rs_plan(R, n);
-  RsLayout L;
+  RsLayout L = {};
+  if (rs_in_a_cluster(R, n)) return L;
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off += align_up(bytes, 256); return o; };
   L.totals = take(4 * kRsBins);
@@ -308,7 +310,7 @@ extern "C" int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_rec
   MLPSP_REQUIRE(R == 0 || (primitive_ids && slots), MLPSP_E_ARG, "%s: null pointer", who);
   MLPSP_REQUIRE(!findings_host || (pixel_offsets && pixels >= 0), MLPSP_E_ARG, "%s: no pixel offsets to check", who);
   const RsLayout L = rs_layout(R, n);
-  MLPSP_REQUIRE(scratch && scratch_bytes >= L.bytes, MLPSP_E_SCRATCH, "%s: scratch needs %lld bytes", who, (long long)L.bytes);
+  MLPSP_REQUIRE(L.bytes == 0 || (scratch && scratch_bytes >= L.bytes), MLPSP_E_SCRATCH, "%s: scratch needs %lld bytes", who, (long long)L.bytes);
   cudaStream_t st = (cudaStream_t)stream;
   HostWords& hw = host_words();
   cudaEvent_t ev = nullptr;
@@ -323,7 +325,7 @@ extern "C" int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_rec
   }
   if (R == 0) {
     MLPSP_CUDA_OK(cudaMemsetAsync(offsets, 0, 8 * ((size_t)n + 1), st));
-  } else if (n < kRsBins && R <= kRsClusterRecords) {
+  } else if (rs_in_a_cluster(R, n)) {
     LaunchScope scope(kKMisc, 1, st);
     constexpr int per_round = kRsClusterCtas * kRsThreads;
     launch_chained(k_rs_cluster, dim3(kRsClusterCtas), dim3(kRsThreads), 0, st, reinterpret_cast<const uint32_t*>(primitive_ids), (int)R, n,

@@ -163,7 +163,6 @@ def _route_args(route):
             route.records, route.offsets.data_ptr() + 8 * (route.offsets.numel() - 1))
 
 
-@torch.no_grad()
 def route_records(primitive_ids: torch.Tensor, num_primitives: int, pixel_offsets: torch.Tensor | None = None, *,
                   check: bool = True) -> RecordRoute:
     """The places of a frame's records among the records grouped by primitive (a stable grouping, as group_records).
@@ -199,7 +198,7 @@ def route_records(primitive_ids: torch.Tensor, num_primitives: int, pixel_offset
     offsets = torch.empty(n + 1, device=dev, dtype=torch.int64)
     slots = torch.empty(R, device=dev, dtype=torch.int32)
     nbytes = int(lib.mlpsp_route_records_scratch_bytes(R, n))
-    scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
     found = C.c_int32(0)
     with _on(dev):
         L.check(lib.mlpsp_route_records(L.ptr(ids), R, n, L.ptr(first), pixels, L.ptr(offsets), L.ptr(slots), L.ptr(scratch), nbytes,

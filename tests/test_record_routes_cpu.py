@@ -28,7 +28,8 @@ def test_c_entries_check_their_arguments():
 
     assert route(R=1 << 31, nbytes=1 << 40) == -4 and route(n=2 ** 31 - 1) == -4 and route(R=-1) == -1
     assert route(slots=None) == -1 and route(ids=None) == -1 and route(offsets=None) == -1
-    assert route(nbytes=8) == -2 and b"scratch needs" in lib.mlpsp_last_error()
+    assert route(n=600, nbytes=8) == -2 and b"scratch needs" in lib.mlpsp_last_error()
+    assert lib.mlpsp_route_records_scratch_bytes(65_536, 511) == 0 and lib.mlpsp_route_records_scratch_bytes(65_537, 511) > 0
     assert route(found=ctypes.byref(ctypes.c_int32())) == -1 and b"no pixel offsets" in lib.mlpsp_last_error()
     assert lib.mlpsp_route_records_scratch_bytes(-1, 3) == -1 and lib.mlpsp_route_records_scratch_bytes(1000, 70_000) > 12_000
     # nothing to do: no launch, no pointer is looked at

@@ -154,9 +154,11 @@ __device__ __forceinline__ void ns_end(const NsArgs& q) {
   if (q.follows) chain_wait();
 }
 
-// matrices of at most kNsWarpRows x kNsWarpCols go to the warp kernel (muon_warp.cu), others to the cluster kernel (muon_tc.cu)
-constexpr int kNsWarpRows = 32, kNsWarpCols = 96;
+// matrices of at most kNsWarpRows x kNsWarpCols go to a warp each (muon_warp.cu), of at most kNsPairRows rows to two (muon_pair.cu), others to
+// a CTA or a cluster (muon_tc.cu)
+constexpr int kNsWarpRows = 32, kNsPairRows = 64, kNsWarpCols = 96;
 int launch_ns_warp(const NsArgs& q, cudaStream_t st);
+int launch_ns_pair(const NsArgs& q, cudaStream_t st);
 int launch_ns_cluster(const NsArgs& q, cudaStream_t st);
 
 }  // namespace mlpsp

@@ -517,7 +517,8 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
   if (!tall)
     for (int v = 2; v <= 4; v *= 2)
       if (cols % v == 0 && wide % (4 * v) == 0 && typed % (size * v) == 0) q.vec = v;
-  return q.small <= kNsWarpRows && q.large <= kNsWarpCols ? launch_ns_warp(q, st) : launch_ns_cluster(q, st);
+  if (q.small > kNsPairRows || q.large > kNsWarpCols) return launch_ns_cluster(q, st);
+  return q.small <= kNsWarpRows ? launch_ns_warp(q, st) : launch_ns_pair(q, st);
 }
 
 }  // namespace mlpsp
@@ -525,7 +526,7 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
 using namespace mlpsp;
 
 extern "C" int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols) {
-  return std::min(rows, cols) > kNsWarpRows || std::max(rows, cols) > kNsWarpCols ? 1 : 0;
+  return std::min(rows, cols) > kNsPairRows || std::max(rows, cols) > kNsWarpCols ? 1 : 0;
 }
 
 extern "C" int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a,

@@ -11,54 +11,9 @@
 // tcgen05 tile of 128 rows would spend three quarters of its products on zeros) and instruction issue, about even.  With X in registers and
 // every loop unrolled the code did not fit the instruction caches: 32 ns per 32 x 72 matrix; so the loops over columns are rolled.
 // Gradient, momentum and weights are read and written once, in fragments (each lane group of four takes a whole 32-byte sector).
-#include "muon.cuh"
+#include "muon_mma.cuh"
 
 namespace mlpsp {
-
-__device__ __forceinline__ void ns_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// the same onto nothing
-__device__ __forceinline__ void ns_mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void ns_mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b0));
-}
-__device__ __forceinline__ uint32_t ns_transpose(uint32_t v) {
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-// 16 rows by 8 N columns at the lane's address: r[2 n + h] = rows 8 h + g, columns 8 n + 2 t; TRANS: the transposes of these 8 x 8 blocks
-template <int N, bool TRANS>
-__device__ __forceinline__ void ns_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
-  if (N == 2) {
-    if (TRANS) asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-    else asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-  } else {
-    if (TRANS) asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
-    else asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
-    r[2] = r[3] = 0u;
-  }
-}
-template <int N>
-__device__ __forceinline__ void ns_stmatrix(uint32_t addr, const uint32_t (&r)[4]) {
-  if (N == 2) asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
-  else asm volatile("stmatrix.sync.aligned.m8n8.x2.shared.b16 [%0], {%1, %2};" ::"r"(addr), "r"(r[0]), "r"(r[1]) : "memory");
-}
-
-// ns_split on the integer and FP32 units: FP32 halves come back from binary16 on half of the multiply-add units only, which were as busy
-// as the tensor cores with ns_split's.  hi: x with its lowest 13 bits rounded off, which binary16 holds exactly down to 2^-14.
-__device__ __forceinline__ float ns_head(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); }
-__device__ __forceinline__ void ns_split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  const float h0 = ns_head(x0), h1 = ns_head(x1);
-  hi = pack_h2<false>(h0, h1);
-  lo = pack_h2<false>(x0 - h0, x1 - h1);
-}
 
 // fragments of a symmetric [16 MB x 16 MB] matrix: f[mb][n][h] = rows 16 mb + 8 h + g, columns 8 n + 2 t and + 1
 template <int MB> struct NsFrag { uint32_t hi[MB][2 * MB][2], lo[MB][2 * MB][2]; };

@@ -42,7 +42,7 @@ def _status(dev, shapes, check):
     if not any(L.load().mlpsp_orthogonalize_waits(rows, cols) for _n, rows, cols in shapes) or not check:
         return None
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("the status of matrices beyond 32 x 96 is read back: pass check=False inside a graph capture")
+        raise RuntimeError("the status of matrices beyond 64 x 96 is read back: pass check=False inside a graph capture")
     return torch.zeros(L.STATUS_WORDS, device=dev, dtype=torch.int32)
 
 
@@ -69,7 +69,7 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     update: float32, float16 or bfloat16, [rows, columns] or [N, rows, columns], contiguous; out (update itself, or a tensor
     apart from it) receives the result in update's type.  The iteration has FP32 accuracy whatever the type.  A matrix of zeros stays
     zero; one that holds an infinity or a NaN becomes NaN and touches no other.  Coefficients under which singular values leave
-    [0, 4] are refused.  Matrices beyond 32 x 96 go to a kernel with bounded waits, whose status is read back unless check is
+    [0, 4] are refused.  Matrices beyond 64 x 96 go to a kernel with bounded waits, whose status is read back unless check is
     False."""
     n, rows, cols = _shape("update", update)
     if update.dtype not in _TYPES:

@@ -451,13 +451,13 @@ int mlpsp_weight_gradients(const mlpsp_scene* scene, const int64_t* offsets, con
  * accuracy whatever the type, and the result is rounded once.  A matrix of zeros gives zeros, one that holds an infinity or a NaN gives
  * NaN, alone.  Coefficients under which singular values leave [0, 4] within the steps are refused, as are more than
  * MLPSP_MUON_MAX_SMALL rows or columns on the shorter and MLPSP_MUON_MAX_LARGE on the longer side; 1e-15 <= eps <= 1, 1 <= steps <= 32.
- * status (or NULL): MLPSP_ST_TIMEOUT when a device-side wait gave up, results then invalid; only shapes for which
- * mlpsp_orthogonalize_waits answers 1 wait. */
+ * gave_up_host (HOST, or NULL) receives 1 when a device-side wait gave up, results then invalid, else 0, for which the call waits; only
+ * shapes for which mlpsp_orthogonalize_waits answers 1 wait. */
 #define MLPSP_MUON_MAX_SMALL 128
 #define MLPSP_MUON_MAX_LARGE 2048
 int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols);
 int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a, double b,
-                        double c, double eps, void* out, int32_t* status, void* stream);
+                        double c, double eps, void* out, int32_t* gave_up_host, void* stream);
 /* One step, in place, on the weight matrices of `count` tensors and their momenta (FP32): m <- m + (1 - momentum)(g - m),
  * U = g + momentum (m - g) (nesterov) or m, w <- (1 - lr weight_decay) w - lr scale X(U), X as above.
  * active [n] (bytes, or NULL; then every tensor's n is the same): matrices whose byte is zero keep weights and momenta and are not
@@ -472,7 +472,7 @@ typedef struct mlpsp_muon_tensor {
   int32_t grad_dtype, reserved0;
 } mlpsp_muon_tensor;
 int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, const uint8_t* active, double lr, double momentum, int32_t nesterov,
-                    double weight_decay, int32_t steps, double a, double b, double c, double eps, int32_t* status, void* stream);
+                    double weight_decay, int32_t steps, double a, double b, double c, double eps, int32_t* gave_up_host, void* stream);
 
 /* ---- the step after the feature map: feature decoder and text query ---- */
 

@@ -22,7 +22,7 @@ struct NsArgs {
   float* w;                  // weights of a step
   void* out;                 // result, in g's type
   const uint8_t* active;     // [count], or null
-  int32_t* status;           // where a wait that gives up says so (the cluster kernel)
+  volatile int32_t* gave_up; // page-locked host word that a wait which gives up sets (the cluster kernel), or null
   int64_t count, stride;     // matrices, elements of each
   int32_t type;              // element type of g and out (MLPSP_PRECISION_*)
   int32_t small, large;      // X is small x large

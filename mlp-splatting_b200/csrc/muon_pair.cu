@@ -6,8 +6,9 @@
 // diagonal a second time transposed.  bA + cA^2 is held as fragments of the warp's rows; X's panels are read by both warps before either
 // writes its rows of them back.
 //
-// A tcgen05 tile holds two such matrices at a time and spends half of its products on the blocks between them; with the passes through
-// tensor memory one 64 x 72 matrix took PLACEHOLDER_TC ns that way, PLACEHOLDER_PAIR ns here (15,000 of them).
+// A tcgen05 tile holds two such matrices at a time and spends half of its products on the blocks between them: with the passes through
+// tensor memory a 64 x 72 matrix took 97 ns of the GPU that way, 57 here (five steps, thousands of matrices), where mma.sync is busy for 70
+// percent of the time.  As in muon_warp.cu small products come before large ones.
 #include "muon_mma.cuh"
 
 namespace mlpsp {
@@ -19,16 +20,17 @@ template <int NB> __host__ __device__ constexpr int np_smem() { return ((NB + 1)
 struct NpBlocks { float d[6][4], o[4][4]; };
 
 // += x x^T over a panel of 8 K columns at `at`; own, top, off: byte offsets of the warp's rows, of row 0 and of row 32 + 16 w
-template <int K>
+// parts PART0 on: hi lo, lo hi, hi hi
+template <int K, int PART0 = 0, int PARTS = 3>
 __device__ __forceinline__ void np_gram(uint32_t xa, uint32_t xb, int own, int off, NpBlocks& b) {
   uint32_t ah[2][4], al[2][4], bh[2][4], bl[2][4], oh[4], ol[4];
 #pragma unroll
   for (int mb = 0; mb < 2; ++mb) {
     ns_ldmatrix<K, false>(ah[mb], xa + own + mb * kNpBlock);
-    ns_ldmatrix<K, false>(al[mb], xa + own + mb * kNpBlock + kNpLo);
+    if (PART0 < 2) ns_ldmatrix<K, false>(al[mb], xa + own + mb * kNpBlock + kNpLo);
     if (K == 2) {
       ns_ldmatrix<K, false>(bh[mb], xb + own + mb * kNpBlock);
-      ns_ldmatrix<K, false>(bl[mb], xb + own + mb * kNpBlock + kNpLo);
+      if (PART0 < 2) ns_ldmatrix<K, false>(bl[mb], xb + own + mb * kNpBlock + kNpLo);
     }
   }
   // word of rows 8 h of a block as the B operand's first or second
@@ -37,7 +39,7 @@ __device__ __forceinline__ void np_gram(uint32_t xa, uint32_t xb, int own, int o
     else ns_mma8(d, l[0], l[1], r[h]);
   };
 #pragma unroll
-  for (int part = 0; part < 3; ++part)
+  for (int part = PART0; part < PART0 + PARTS; ++part)
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -49,12 +51,12 @@ __device__ __forceinline__ void np_gram(uint32_t xa, uint32_t xb, int own, int o
 #pragma unroll
   for (int mb = 0; mb < 2; ++mb) {
     ns_ldmatrix<K, false>(ah[mb], xa + mb * kNpBlock);
-    ns_ldmatrix<K, false>(al[mb], xa + mb * kNpBlock + kNpLo);
+    if (PART0 < 2) ns_ldmatrix<K, false>(al[mb], xa + mb * kNpBlock + kNpLo);
   }
   ns_ldmatrix<K, false>(oh, (K == 2 ? xb : xa) + off);
-  ns_ldmatrix<K, false>(ol, (K == 2 ? xb : xa) + off + kNpLo);
+  if (PART0 < 2) ns_ldmatrix<K, false>(ol, (K == 2 ? xb : xa) + off + kNpLo);
 #pragma unroll
-  for (int part = 0; part < 3; ++part)
+  for (int part = PART0; part < PART0 + PARTS; ++part)
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -253,7 +255,9 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
 #pragma unroll
       for (int i = 0; i < 4; ++i) S.o[i][0] = S.o[i][1] = S.o[i][2] = S.o[i][3] = 0.f;
 #pragma unroll 1
-      for (int p = 0; p < 4; ++p) np_gram<2>(aa + p * kNpPanel, ab + p * kNpPanel, own, off, S);
+      for (int p = 0; p < 4; ++p) np_gram<2, 0, 2>(aa + p * kNpPanel, ab + p * kNpPanel, own, off, S);
+#pragma unroll 1
+      for (int p = 0; p < 4; ++p) np_gram<2, 2, 1>(aa + p * kNpPanel, ab + p * kNpPanel, own, off, S);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -285,23 +289,33 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
       // ---- X <- a X + P X, a panel at a time
       auto product = [&](int p, auto width, float (&e)[2][2][4]) {
         constexpr int N = decltype(width)::value;
+        uint32_t bh[4][4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t bh[4], bl[4];
-          ns_ldmatrix<N, true>(bh, xa + p * kNpPanel + c * kNpBlock);
+          uint32_t bl[4];
+          ns_ldmatrix<N, true>(bh[c], xa + p * kNpPanel + c * kNpBlock);
           ns_ldmatrix<N, true>(bl, xa + p * kNpPanel + c * kNpBlock + kNpLo);
 #pragma unroll
-          for (int part = 0; part < 3; ++part)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+            for (int mb = 0; mb < 2; ++mb) {
+              const uint32_t(&l)[4] = ph[mb][c];
+              if (c == 0) ns_mma_first(e[mb][n], l[0], l[1], l[2], l[3], bl[2 * n], bl[2 * n + 1]);
+              else ns_mma(e[mb][n], l[0], l[1], l[2], l[3], bl[2 * n], bl[2 * n + 1]);
+            }
 #pragma unroll
-              for (int mb = 0; mb < 2; ++mb) {
-                const uint32_t(&l)[4] = part == 1 ? pl[mb][c] : ph[mb][c];
-                const uint32_t(&r)[4] = part == 0 ? bl : bh;
-                if (c == 0 && part == 0) ns_mma_first(e[mb][n], l[0], l[1], l[2], l[3], r[2 * n], r[2 * n + 1]);
-                else ns_mma(e[mb][n], l[0], l[1], l[2], l[3], r[2 * n], r[2 * n + 1]);
-              }
+          for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int mb = 0; mb < 2; ++mb)
+              ns_mma(e[mb][n], pl[mb][c][0], pl[mb][c][1], pl[mb][c][2], pl[mb][c][3], bh[c][2 * n], bh[c][2 * n + 1]);
         }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int mb = 0; mb < 2; ++mb)
+              ns_mma(e[mb][n], ph[mb][c][0], ph[mb][c][1], ph[mb][c][2], ph[mb][c][3], bh[c][2 * n], bh[c][2 * n + 1]);
       };
       // rows of block mb: the new values
       auto advance = [&](int mb, int p, auto width, const float (&e)[2][2][4], float (&v)[2][2][2]) {

@@ -6,7 +6,7 @@
 // computed by each.  Narrow matrices of few rows are stacked (two of 64 rows): the blocks of A off their diagonal are cleared, after
 // which everything stays block-diagonal.  Accumulators (A | A^2, later the new slice in the same columns) are in tensor memory.
 //
-// Every wait on an mbarrier is bounded; one that gives up raises MLPSP_ST_TIMEOUT and this CTA's slice of the result is not written.
+// Every wait on an mbarrier is bounded; one that gives up is reported to the host, and this CTA's slice of the result is not written.
 #include <cmath>
 #include "muon.cuh"
 
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
       ready();
     }
   }
-  if (!ok && q.status) atomicOr(q.status + MLPSP_ST_BITS, MLPSP_ST_TIMEOUT);
+  if (!ok && q.gave_up) *q.gave_up = 1;
   __syncthreads();
   if (warp == 0) tmem_free(tmem, kNtTmemCols);
   if (cluster > 1) nt_cluster_sync();      // no CTA leaves while another may read its shared memory
@@ -525,40 +525,73 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
 
 using namespace mlpsp;
 
+namespace mlpsp {
+// the answer of a call's waits, for which the call waits
+struct NsAnswer {
+  int32_t* to;
+  HostWords& hw;
+  cudaEvent_t ev = nullptr;
+  explicit NsAnswer(int32_t* host) : to(host), hw(host_words()) {}
+  int open(NsArgs& q) {
+    if (!to) return MLPSP_OK;
+    const int rc = hw.open(&ev);
+    if (rc) return rc;
+    hw.word[0] = 0;
+    q.gave_up = static_cast<volatile int32_t*>(hw.word);
+    return MLPSP_OK;
+  }
+  int read(cudaStream_t st) {
+    if (!to) return MLPSP_OK;
+    MLPSP_CUDA_OK(cudaEventRecord(ev, st));
+    MLPSP_CUDA_OK(cudaEventSynchronize(ev));
+    *to = *static_cast<volatile int32_t*>(hw.word);
+    return MLPSP_OK;
+  }
+};
+}  // namespace mlpsp
+
 extern "C" int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols) {
   return std::min(rows, cols) > kNsPairRows || std::max(rows, cols) > kNsWarpCols ? 1 : 0;
 }
 
 extern "C" int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a,
-                                   double b, double c, double eps, void* out, int32_t* status, void* stream) {
+                                   double b, double c, double eps, void* out, int32_t* gave_up_host, void* stream) {
   NsArgs q = {};
   q.g = update;
   q.out = out;
   q.type = dtype;
-  q.status = status;
-  return ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream);
+  NsAnswer answer(gave_up_host);
+  int rc = ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream, false);
+  if (!rc) rc = answer.open(q);
+  if (!rc) rc = ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream);
+  return rc ? rc : answer.read((cudaStream_t)stream);
 }
 
 extern "C" int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, const uint8_t* active, double lr, double momentum,
                                int32_t nesterov, double weight_decay, int32_t steps, double a, double b, double c, double eps,
-                               int32_t* status, void* stream) {
+                               int32_t* gave_up_host, void* stream) {
   MLPSP_REQUIRE(count >= 0 && (count == 0 || tensors), MLPSP_E_ARG, "mlpsp_muon_step: null pointer");
   MLPSP_REQUIRE(momentum >= 0.0 && momentum < 1.0, MLPSP_E_ARG, "mlpsp_muon_step: momentum must be within [0, 1)");
   MLPSP_REQUIRE(lr >= 0.0 && lr < 1e30 && weight_decay >= 0.0 && weight_decay < 1e30, MLPSP_E_ARG,
                 "mlpsp_muon_step: lr and weight_decay must be finite and not negative");
+  NsAnswer answer(gave_up_host);
   for (int pass = 0; pass < 2; ++pass) {       // all tensors are checked before the first launch
     bool follows = false;
+    NsArgs shared = {};
+    if (pass == 1) {
+      const int rc = answer.open(shared);
+      if (rc) return rc;
+    }
     for (int32_t i = 0; i < count; ++i) {
       const mlpsp_muon_tensor& t = tensors[i];
       MLPSP_REQUIRE(t.n <= 0 || (t.weights && t.grads && t.momenta), MLPSP_E_ARG, "mlpsp_muon_step: null pointer");
       MLPSP_REQUIRE(t.scale > 0.0 && t.scale < 1e30, MLPSP_E_ARG, "mlpsp_muon_step: scale must be finite and positive");
-      NsArgs q = {};
+      NsArgs q = shared;
       q.g = t.grads;
       q.m = t.momenta;
       q.w = t.weights;
       q.active = active;
       q.type = t.grad_dtype;
-      q.status = status;
       q.nesterov = nesterov != 0;
       q.momentum = (float)momentum;
       q.rest = (float)(1.0 - momentum);
@@ -570,5 +603,5 @@ extern "C" int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, 
       follows |= t.n > 0;
     }
   }
-  return MLPSP_OK;
+  return answer.read((cudaStream_t)stream);
 }

@@ -35,11 +35,11 @@ __device__ __forceinline__ void ns_mirror(NsFrag<MB>& s) {
 // same words with those of a row next to each other, as B operands want them (K = 1: the same).  The blocks
 // advance together, since an MMA takes four times as long to answer as to issue; small products first, so that the tensor core's
 // rounding of a sum towards zero meets fewer large ones.
-template <int MB, int K, bool FIRST>
+template <int MB, int K, bool FIRST, int PART0 = 0, int PARTS = 3>
 __device__ __forceinline__ void ns_gram(const uint32_t (&ah)[MB][4], const uint32_t (&al)[MB][4], const uint32_t (&bh)[MB][4],
                                         const uint32_t (&bl)[MB][4], float (&d)[MB * (MB + 1)][4]) {
 #pragma unroll
-  for (int part = 0; part < 3; ++part) {
+  for (int part = PART0; part < PART0 + PARTS; ++part) {
     const auto& l = part == 1 ? al : ah;
     const auto& r = part == 0 ? bl : bh;
 #pragma unroll
@@ -336,20 +336,23 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
       // ---- P = b A + c A^2.  Its diagonal is kept apart and multiplies X in FP32 below: the rest is smaller, and with it what the tensor
       // core's rounding towards zero takes off (4e-6 of the result for 128 rows with the diagonal in, 2e-6 so)
 #pragma unroll
-      for (int k = 0; k < MB; ++k) {
-        uint32_t hi[MB][4], lo[MB][4], bh[MB][4], bl[MB][4];
+      for (int round = 0; round < 2; ++round)
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
+        for (int k = 0; k < MB; ++k) {
+          uint32_t hi[MB][4], lo[MB][4], bh[MB][4], bl[MB][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            hi[mb][i] = A.hi[mb][2 * k + (i >> 1)][i & 1];
-            lo[mb][i] = A.lo[mb][2 * k + (i >> 1)][i & 1];
-            bh[mb][i] = A.hi[mb][2 * k + (i & 1)][i >> 1];
-            bl[mb][i] = A.lo[mb][2 * k + (i & 1)][i >> 1];
-          }
-        if (k == 0) ns_gram<MB, 2, true>(hi, lo, bh, bl, d);
-        else ns_gram<MB, 2, false>(hi, lo, bh, bl, d);
-      }
+          for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              hi[mb][i] = A.hi[mb][2 * k + (i >> 1)][i & 1];
+              lo[mb][i] = A.lo[mb][2 * k + (i >> 1)][i & 1];
+              bh[mb][i] = A.hi[mb][2 * k + (i & 1)][i >> 1];
+              bl[mb][i] = A.lo[mb][2 * k + (i & 1)][i >> 1];
+            }
+          if (round == 1) ns_gram<MB, 2, false, 2, 1>(hi, lo, bh, bl, d);
+          else if (k == 0) ns_gram<MB, 2, true, 0, 2>(hi, lo, bh, bl, d);
+          else ns_gram<MB, 2, false, 0, 2>(hi, lo, bh, bl, d);
+        }
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll

@@ -7,6 +7,7 @@ own rule.  There is no CPU path.
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 
 import torch
@@ -37,17 +38,17 @@ def _check_tensors(tensors):
     return dev
 
 
-def _status(dev, shapes, check):
-    """A status block for calls whose kernels wait on the device, or None."""
-    if not any(L.load().mlpsp_orthogonalize_waits(rows, cols) for _n, rows, cols in shapes) or not check:
+def _answer(shapes, check):
+    """A word for the answer of kernels that wait on the device, or None."""
+    if not check or not any(L.load().mlpsp_orthogonalize_waits(rows, cols) for _n, rows, cols in shapes):
         return None
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("the status of matrices beyond 64 x 96 is read back: pass check=False inside a graph capture")
-    return torch.zeros(L.STATUS_WORDS, device=dev, dtype=torch.int32)
+        raise RuntimeError("matrices beyond 64 x 96 wait for the kernel's answer: pass check=False inside a graph capture")
+    return C.c_int32(0)
 
 
-def _read_status(status, what):
-    if status is not None and int(status[L.ST_BITS].item()) & L.BIT_TIMEOUT:
+def _read(answer, what):
+    if answer is not None and answer.value:
         raise RuntimeError(f"{what}: a device-side wait gave up; results are invalid")
 
 
@@ -69,8 +70,8 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     update: float32, float16 or bfloat16, [rows, columns] or [N, rows, columns], contiguous; out (update itself, or a tensor
     apart from it) receives the result in update's type.  The iteration has FP32 accuracy whatever the type.  A matrix of zeros stays
     zero; one that holds an infinity or a NaN becomes NaN and touches no other.  Coefficients under which singular values leave
-    [0, 4] are refused.  Matrices beyond 64 x 96 go to a kernel with bounded waits, whose status is read back unless check is
-    False."""
+    [0, 4] are refused.  Matrices beyond 64 x 96 go to a kernel with bounded waits, for whose answer the call waits
+    unless check is False."""
     n, rows, cols = _shape("update", update)
     if update.dtype not in _TYPES:
         raise ValueError("update must be float32, float16 or bfloat16")
@@ -81,10 +82,10 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
         raise ValueError("out must have the shape and type of update")
     dev = _check_tensors([update, out])
     with _on(dev):
-        status = _status(dev, [(n, rows, cols)], check)
-        L.check(L.load().mlpsp_orthogonalize(L.ptr(update), _TYPES[update.dtype], n, rows, cols, *args, L.ptr(out), L.ptr(status),
-                                             _stream_ptr(dev)), "mlpsp_orthogonalize")
-        _read_status(status, "orthogonalize")
+        answer = _answer([(n, rows, cols)], check)
+        L.check(L.load().mlpsp_orthogonalize(L.ptr(update), _TYPES[update.dtype], n, rows, cols, *args, L.ptr(out),
+                                             None if answer is None else C.byref(answer), _stream_ptr(dev)), "mlpsp_orthogonalize")
+    _read(answer, "orthogonalize")
     return out
 
 
@@ -130,10 +131,10 @@ def muon_step(weights, grads, momenta, *, lr: float, momentum: float = 0.95, nes
         reached[1] = max(reached[1], end if written else 0)
     lib = L.load()
     with _on(dev):
-        status, st = _status(dev, shapes, check), _stream_ptr(dev)
+        answer = _answer(shapes, check)
         tensors = (L.MuonTensor * len(shapes))(*(
             (L.ptr(w), L.ptr(g), L.ptr(m), n, rows, cols, math.sqrt(max(1.0, rows / cols)), _TYPES[g.dtype], 0)
             for w, g, m, (n, rows, cols) in zip(*lists, shapes)))
         L.check(lib.mlpsp_muon_step(tensors, len(shapes), L.ptr(active), lr, momentum, int(bool(nesterov)), weight_decay, *args,
-                                    L.ptr(status), st), "mlpsp_muon_step")
-        _read_status(status, "muon_step")
+                                    None if answer is None else C.byref(answer), _stream_ptr(dev)), "mlpsp_muon_step")
+    _read(answer, "muon_step")

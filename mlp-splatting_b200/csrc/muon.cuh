@@ -154,9 +154,13 @@ __device__ __forceinline__ void ns_end(const NsArgs& q) {
   if (q.follows) chain_wait();
 }
 
-// matrices of at most kNsWarpRows x kNsWarpCols go to a warp each (muon_warp.cu), of at most kNsPairRows rows to two (muon_pair.cu), others to
-// a CTA or a cluster (muon_tc.cu)
-constexpr int kNsWarpRows = 32, kNsPairRows = 64, kNsWarpCols = 96;
+// Which kernel: a warp for matrices of up to 32 rows (muon_warp.cu), two for up to 64 (muon_pair.cu), a CTA or a cluster for the rest
+// (muon_tc.cu).  Up to kNsFew columns the first two are as fast with a single matrix and faster with many; beyond, a cluster is done sooner
+// with few but its 128 rows are mostly empty, so they take over once the clusters would go round more than twice, as far as a warp's or
+// pair's X fits an SM's shared memory.
+constexpr int kNsWarpRows = 32, kNsPairRows = 64;
+constexpr int kNsWarpFew = 512, kNsPairFew = 256;
+constexpr int kNsWarpLong[2] = {2048, 1024}, kNsPairLong = 512;       // warp: up to 16 rows, up to 32
 int launch_ns_warp(const NsArgs& q, cudaStream_t st);
 int launch_ns_pair(const NsArgs& q, cudaStream_t st);
 int launch_ns_cluster(const NsArgs& q, cudaStream_t st);

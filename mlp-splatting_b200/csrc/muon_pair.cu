@@ -1,4 +1,4 @@
-// Newton-Schulz iteration of matrices of 33 to 64 rows and at most 96 columns (64-wide layers of a primitive), two warps per matrix.
+// Newton-Schulz iteration of matrices of 33 to 64 rows (64-wide layers of a primitive among them), two warps per matrix.
 //
 // The scheme of muon_warp.cu for twice the rows: X and A lie in shared memory as binary16 pairs in panels of 16 columns, warp w has the
 // rows 32 w to 32 w + 31.  Of A and A^2 a warp computes the blocks of its own rows on and below the diagonal (six of 16 x 8) and half of the
@@ -14,7 +14,7 @@
 namespace mlpsp {
 
 constexpr int kNpThreads = 64, kNpRows = 64, kNpPanel = kNpRows * 64, kNpLo = kNpPanel / 2, kNpBlock = 16 * 32;
-template <int NB> __host__ __device__ constexpr int np_smem() { return ((NB + 1) / 2 + 4) * kNpPanel + 32; }
+__host__ __device__ constexpr int np_smem(int panels) { return (panels + 4) * kNpPanel + 32; }
 
 // d: blocks (mb, n), n <= 2 mb + 1, of the warp's own rows at mb (mb + 1) + n; o: blocks (mb, n) of rows 16 mb, columns 32 + 16 w + 8 n at 2 mb + n
 struct NpBlocks { float d[6][4], o[4][4]; };
@@ -87,7 +87,7 @@ __device__ __forceinline__ void np_put(uint32_t sa, int w, const NpBlocks& b) {
 
 template <int NB, int CTAS>
 __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, const bool prefetch) {
-  constexpr int kPanels = (NB + 1) / 2;
+  const int kPanels = NB ? (NB + 1) / 2 : (q.large + 15) / 16, kWhole = NB ? NB / 2 : kPanels;      // kWhole: of two columns of blocks
   extern __shared__ __align__(128) char smem[];
   ns_begin(q);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, w = warp_of_cta();
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
       const bool stepping = V == 1 ? q.m != nullptr : STEP;
 #pragma unroll 1
       for (int p = 0; p < kPanels; ++p) {
-        float v[2][2][2][2], m[2][2][2][2];
+        float v[2][2][2][2], m[2][2][2][2], part = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -161,9 +161,10 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
                     ns_store<V>(q.m, base(mb, h) + (V == 2 ? (int64_t)col : (int64_t)col * q.cs), MLPSP_PRECISION_F32, n);
                 }
               }
-              squares = fmaf(x[0], x[0], fmaf(x[1], x[1], squares));
+              part = fmaf(x[0], x[0], fmaf(x[1], x[1], part));
               keep(p, u, mb, h) = make_float2(x[0], x[1]);
             }
+        squares += part;
       }
     };
     if (q.vec >= 2) {
@@ -237,8 +238,25 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
       for (int i = 0; i < 6; ++i) A.d[i][0] = A.d[i][1] = A.d[i][2] = A.d[i][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) A.o[i][0] = A.o[i][1] = A.o[i][2] = A.o[i][3] = 0.f;
+      if (NB) {
 #pragma unroll 1
-      for (int p = 0; p < NB / 2; ++p) np_gram<2>(xa + p * kNpPanel, xb + p * kNpPanel, own, off, A);
+        for (int p = 0; p < kWhole; ++p) np_gram<2>(xa + p * kNpPanel, xb + p * kNpPanel, own, off, A);
+      } else {
+        // long rows two panels at a time (muon_warp.cu)
+#pragma unroll 1
+        for (int p0 = 0; p0 < kWhole; p0 += 2) {
+          NpBlocks part = {};
+#pragma unroll 1
+          for (int p = p0; p < min(p0 + 2, kWhole); ++p) np_gram<2>(xa + p * kNpPanel, xb + p * kNpPanel, own, off, part);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) A.d[i][e] += part.d[i][e];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) A.o[i][e] += part.o[i][e];
+          }
+        }
+      }
       if (NB & 1) np_gram<1>(xa + NB / 2 * kNpPanel, xb + NB / 2 * kNpPanel, own, off, A);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -351,7 +369,7 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
         float e[2][2][4], next[2][2][4];
         product(0, NsTag<2>{}, e);
 #pragma unroll 1
-        for (int p = 1; p < NB / 2; ++p) {
+        for (int p = 1; p < kWhole; ++p) {
           __syncthreads();       // both warps have read panel p - 1
           product(p, NsTag<2>{}, next);
           store(p - 1, NsTag<2>{}, e);
@@ -362,7 +380,7 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
         }
         __syncthreads();
         if (NB & 1) product(NB / 2, NsTag<1>{}, next);
-        store(NB / 2 - 1, NsTag<2>{}, e);
+        store(kWhole - 1, NsTag<2>{}, e);
         if (NB & 1) {
           __syncthreads();
           store(NB / 2, NsTag<1>{}, next);
@@ -409,7 +427,7 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
         }
       };
 #pragma unroll 1
-      for (int p = 0; p < NB / 2; ++p) finish(p, NsTag<2>{});
+      for (int p = 0; p < kWhole; ++p) finish(p, NsTag<2>{});
       if (NB & 1) finish(NB / 2, NsTag<1>{});
     }
   };
@@ -419,10 +437,11 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
 
 template <int NB, int CTAS>
 static int ns_pair(const NsArgs& q, cudaStream_t st) {
-  constexpr int smem = np_smem<NB>();
-  static_assert(CTAS * (smem + 1024) <= 227 * 1024, "resident CTAs");
+  constexpr int most = np_smem(NB ? (NB + 1) / 2 : kNsPairLong / 16);
+  static_assert(most <= 227 * 1024 && (NB == 0 || CTAS * (most + 1024) <= 227 * 1024), "resident CTAs");
+  const int smem = NB ? most : np_smem((q.large + 15) / 16);
   static DeviceOnce once;
-  if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_pair<NB, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_pair<NB, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
   MLPSP_REQUIRE(q.count < (1ll << 31), MLPSP_E_LIMIT, "orthogonalize: too many matrices");
   const bool prefetch = reinterpret_cast<uintptr_t>(q.w) % 16 == 0 && q.stride % 4 == 0;
   LaunchScope scope(kKMisc, 1, st);
@@ -431,7 +450,7 @@ static int ns_pair(const NsArgs& q, cudaStream_t st) {
 
 int launch_ns_pair(const NsArgs& q, cudaStream_t st) {
   const int nb = (q.large + 7) / 8;
-  return nb <= 6 ? ns_pair<6, 6>(q, st) : nb <= 8 ? ns_pair<8, 6>(q, st) : nb <= 9 ? ns_pair<9, 6>(q, st) : ns_pair<12, 5>(q, st);
+  return nb <= 6 ? ns_pair<6, 6>(q, st) : nb <= 8 ? ns_pair<8, 6>(q, st) : nb <= 9 ? ns_pair<9, 6>(q, st) : nb <= 12 ? ns_pair<12, 5>(q, st) : ns_pair<0, 6>(q, st);
 }
 
 }  // namespace mlpsp

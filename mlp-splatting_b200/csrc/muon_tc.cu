@@ -3,8 +3,8 @@
 // A CTA holds a slice of X, 128 rows by up to 256 columns, in shared memory as binary16 pairs, in chunks of [128 rows][8 columns].
 // The same bytes are the K-major operands of A = X X^T and, read MN-major, the B operand of (bA + cA^2) X.  A matrix of more columns
 // than one slice is spread over a cluster of up to eight CTAs, which add their parts of A through distributed shared memory; A^2 is
-// computed by each.  Narrow matrices of few rows are stacked (two of 64 rows): the blocks of A off their diagonal are cleared, after
-// which everything stays block-diagonal.  Accumulators (A | A^2, later the new slice in the same columns) are in tensor memory.
+// computed by each.  Matrices of few rows are stacked (four of 32): the blocks of A off their diagonal are cleared, after which
+// everything stays block-diagonal.  Accumulators (A | A^2, later the new slice in the same columns) are in tensor memory.
 //
 // Every wait on an mbarrier is bounded; one that gives up is reported to the host, and this CTA's slice of the result is not written.
 #include <cmath>
@@ -19,7 +19,7 @@ constexpr int kNtTmemCols = 256;
 constexpr uint32_t kNtMnB = 1u << 16;      // bit 16 of the instruction descriptor: B is MN-major
 
 // shared memory: X hi | X lo (NP / 8 chunks each) | A hi | A lo (16 chunks each; the FP32 parts of A pass through here too) | small
-constexpr int kNtSmall = kNtParts * kNtRows * 16 + (kNtRows + 1) * 16 + 64;
+constexpr int kNtSmall = (kNtParts + 1) * kNtRows * 16 + 64;
 __host__ __device__ constexpr int nt_smem(int np) { return np * (2 * kNtChunk / 8) + 32 * kNtChunk + kNtSmall; }
 static_assert(nt_smem(kNtMaxCols) <= 227 * 1024, "a CTA's shared memory");
 
@@ -57,7 +57,7 @@ __device__ __forceinline__ void nt_get(const char* hi, const char* lo, float (&x
   }
 }
 
-// `np` columns per CTA, `pack` matrices per tile (1 in a cluster)
+// `np` columns per CTA, `pack` matrices per tile
 __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const int np, const int cluster, const int pack, const int64_t tiles) {
   ns_begin(q);
   extern __shared__ __align__(1024) char smem[];
@@ -69,15 +69,14 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
   char* const pxl = pxh + np * (kNtChunk / 8);
   char* const pah = pxl + np * (kNtChunk / 8);
   char* const pal = pah + 16 * kNtChunk;
-  // [4][128] squares of a row's parts: plain, shrunk, grown | [128] sums of the tile's matrices | this CTA's, read by the cluster's others
+  // [4][128] squares of a row's parts: plain, shrunk, grown | [128] sums of the tile's matrices, read by the cluster's others too
   float4* const s_part = reinterpret_cast<float4*>(smem + np * (2 * kNtChunk / 8) + 32 * kNtChunk);
   float4* const s_sum = s_part + kNtParts * kNtRows;
-  float4* const s_rank = s_sum + kNtRows;
   // between the norms: [128] the diagonal of A, and [4][128] each the parts' sums of squares of a row of X and of A
   float* const s_diag = reinterpret_cast<float*>(s_sum);
   float* const s_xsq = reinterpret_cast<float*>(s_part);
   float* const s_asq = s_xsq + kNtParts * kNtRows;
-  uint32_t* const s_word = reinterpret_cast<uint32_t*>(s_rank + 1);           // mbarrier (two words) | tensor memory | gave up
+  uint32_t* const s_word = reinterpret_cast<uint32_t*>(s_sum + kNtRows);           // mbarrier (two words) | tensor memory | gave up
   const uint32_t bar = smem_u32(s_word);
   uint32_t rank = 0u;
   if (cluster > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -132,7 +131,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
     const int64_t k = tile * pack + sub;
     const bool in = sub < pack && k < q.count && (!q.active || q.active[k]);
     const int64_t base = in ? k * q.stride + (int64_t)srow * q.rs : 0;
-    if (!__syncthreads_or(in)) continue;         // the same answer in every CTA of a cluster: it holds one matrix
+    if (!__syncthreads_or(in)) continue;         // the same answer in every CTA of a cluster: they hold slices of the same matrices
     // ---- momentum, and the update's values in FP32 in the places of X's pairs (eight to a pair of 16-byte words); sums of squares
     float4 ss = make_float4(0.f, 0.f, 0.f, 0.f);
     auto load = [&](auto width) {
@@ -197,10 +196,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
         sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
         sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o);
       }
-      if ((tid & 31) == 0) {
-        s_sum[p] = sum;
-        if (p == 0) *s_rank = sum;
-      }
+      if ((tid & 31) == 0) s_sum[p] = sum;
     }
     if (cluster > 1) nt_cluster_sync();
     else __syncthreads();
@@ -209,7 +205,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
       float4 o[kNtMaxCluster];
 #pragma unroll
       for (int r = 0; r < kNtMaxCluster; ++r)
-        if (r < cluster) o[r] = nt_peer_load(nt_map(smem_u32(s_rank), r));
+        if (r < cluster) o[r] = nt_peer_load(nt_map(smem_u32(s_sum + min(sub, pack - 1)), r));
 #pragma unroll
       for (int r = 0; r < kNtMaxCluster; ++r)
         if (r < cluster) { sum.x += o[r].x; sum.y += o[r].y; sum.z += o[r].z; }
@@ -317,11 +313,16 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int gr = part + j * kNtParts;
+          const int first = gr * 16 - row + srow;       // column of the first value in this row's block of A
           uint32_t h[8], l[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            ns_split(t[j][e].x * by.gram, t[j][e].y * by.gram, h[2 * e], l[2 * e]);
-            ns_split(t[j][e].z * by.gram, t[j][e].w * by.gram, h[2 * e + 1], l[2 * e + 1]);
+            const float a[4] = {t[j][e].x, t[j][e].y, t[j][e].z, t[j][e].w};
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = (unsigned)(first + 4 * e + i) < (unsigned)q.small ? a[i] * by.gram : 0.f;
+            ns_split(v[0], v[1], h[2 * e], l[2 * e]);
+            ns_split(v[2], v[3], h[2 * e + 1], l[2 * e + 1]);
           }
           nt_put(pah + gr * 2 * kNtChunk, pal + gr * 2 * kNtChunk, h, l);
         }
@@ -435,11 +436,15 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
   ns_end(q);
 }
 
+// CTAs that share a matrix: slices of 64 to 128 columns (to 256 beyond 1,024), since the exchange costs as much as the products it spreads
+static int nt_cluster(int large) { return std::min(kNtMaxCluster, std::max(1, (large + 127) / 128)); }
+// whether the tiles need more than two rounds of all clusters
+static bool ns_many(const NsArgs& q) { return (q.count + kNtRows / q.small - 1) / (kNtRows / q.small) > 2 * (int64_t)(sm_count() / nt_cluster(q.large)); }
+
 int launch_ns_cluster(const NsArgs& q, cudaStream_t st) {
-  // columns per CTA: slices of at least 64 (below, the exchange costs more than the products it spreads), at most 256
-  const int cluster = std::min(kNtMaxCluster, std::max(1, (q.large + 127) / 128));
+  const int cluster = nt_cluster(q.large);
   const int np = ((q.large + cluster - 1) / cluster + 15) / 16 * 16;
-  const int pack = cluster == 1 ? kNtRows / q.small : 1;
+  const int pack = kNtRows / q.small;
   const int64_t tiles = (q.count + pack - 1) / pack;
   const int smem = nt_smem(np);
   static DeviceOnce once;
@@ -517,8 +522,12 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
   if (!tall)
     for (int v = 2; v <= 4; v *= 2)
       if (cols % v == 0 && wide % (4 * v) == 0 && typed % (size * v) == 0) q.vec = v;
-  if (q.small > kNsPairRows || q.large > kNsWarpCols) return launch_ns_cluster(q, st);
-  return q.small <= kNsWarpRows ? launch_ns_warp(q, st) : launch_ns_pair(q, st);
+  if (q.small <= kNsWarpRows) {
+    if (q.large <= kNsWarpFew || (q.large <= kNsWarpLong[q.small > 16] && ns_many(q))) return launch_ns_warp(q, st);
+  } else if (q.small <= kNsPairRows) {
+    if (q.large <= kNsPairFew || (q.large <= kNsPairLong && ns_many(q))) return launch_ns_pair(q, st);
+  }
+  return launch_ns_cluster(q, st);
 }
 
 }  // namespace mlpsp
@@ -551,7 +560,8 @@ struct NsAnswer {
 }  // namespace mlpsp
 
 extern "C" int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols) {
-  return std::min(rows, cols) > kNsPairRows || std::max(rows, cols) > kNsWarpCols ? 1 : 0;
+  const int small = std::min(rows, cols), large = std::max(rows, cols);
+  return small > kNsPairRows || large > (small <= kNsWarpRows ? kNsWarpFew : kNsPairFew) ? 1 : 0;
 }
 
 extern "C" int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a,

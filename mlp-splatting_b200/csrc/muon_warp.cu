@@ -1,4 +1,4 @@
-// Newton-Schulz iteration of small matrices (at most 32 x 96: the layers of a primitive), a warp per tile of 16 or 32 rows.
+// Newton-Schulz iteration of matrices of at most 32 rows (the layers of a primitive among them), a warp per tile of 16 or 32 rows.
 //
 // X lies in the warp's shared memory as binary16 pairs, in panels of 16 columns, A and bA + cA^2 in its registers as fragments of m16n8 tiles (lane
 // 4 g + t: rows g and g + 8, columns 2 t and 2 t + 1), in which form a symmetric matrix is at once an A and a B operand.  ldmatrix gives X
@@ -58,7 +58,6 @@ __device__ __forceinline__ void ns_gram(const uint32_t (&ah)[MB][4], const uint3
 // A panel: hi [16 MB rows][16 columns], then lo; the two 16-byte halves of a row change places every four rows, so that eight rows of
 // one half lie in different banks.  It takes the bytes of its values in FP32, as which they arrive.
 template <int MB> __host__ __device__ constexpr int ns_panel_bytes() { return 16 * MB * 64; }
-template <int MB, int NB> __host__ __device__ constexpr int ns_warp_smem() { return (NB + 1) / 2 * ns_panel_bytes<MB>(); }
 
 // brings the `n` elements at element i of an array of `size`-byte elements into L2 (addresses and sizes are multiples of 16 bytes)
 __device__ __forceinline__ void ns_prefetch(const void* p, int64_t i, int n, int size) {
@@ -69,16 +68,15 @@ __device__ __forceinline__ void ns_prefetch(const void* p, int64_t i, int n, int
 // slowest SM set the time and its warps fell into step, all loading and then all multiplying: a step of 100,000 matrices of 32 x 72
 // 2,540 us, now 1,720 (of which 704 are its bytes).  prefetch: a tile's weights, wanted last, are brought into L2 when it starts (1,817
 // without).  Twenty warps per SM instead of sixteen: 2,160.
-constexpr int kNsWarps = 1;       // per CTA: places fall free one by one
-
 template <int MB, int NB, int CTAS>
-__global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(const NsArgs q, const int pack, const int64_t tiles, const bool prefetch) {
+__global__ void __launch_bounds__(32, CTAS) k_ns_warp(const NsArgs q, const int pack, const bool prefetch) {
   constexpr int KH = MB == 1 ? 2 : 1;       // with one block of rows, rows h = 0 and 1 of a lane may belong to two matrices
-  constexpr int kPanels = (NB + 1) / 2, kPanel = ns_panel_bytes<MB>(), kLo = kPanel / 2, kBlock = 16 * 32;
+  constexpr int kPanel = ns_panel_bytes<MB>(), kLo = kPanel / 2, kBlock = 16 * 32;
+  const int kPanels = NB ? (NB + 1) / 2 : (q.large + 15) / 16, kWhole = NB ? NB / 2 : kPanels;      // kWhole: of two columns of blocks
   extern __shared__ __align__(128) char smem[];
   ns_begin(q);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  char* const mine = smem + (threadIdx.x >> 5) * ns_warp_smem<MB, NB>();
+  char* const mine = smem;
   const uint32_t xs = smem_u32(mine);
   // this lane's row of the 8 x 8 blocks that ldmatrix and stmatrix name: lanes 0-7 rows 0-7, 8-15 rows 8-15, 16-31 the same, 8 columns on
   const uint32_t xa = xs + (lane & 15) * 32 + (((lane >> 4) ^ ((lane >> 2) & 1)) << 4);
@@ -99,9 +97,8 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
 #pragma unroll
         for (int e = 0; e < 2; ++e) same |= (sub[h] == (n * 8 + 2 * t + e) / q.small ? 1u : 0u) << (h * 4 + n * 2 + e);
   }
-  const int64_t tile = (int64_t)blockIdx.x * kNsWarps + (threadIdx.x >> 5);
+  const int64_t tile = blockIdx.x;
   auto work = [&] {
-    if (tile >= tiles) return;
     // element of the first column of this lane's rows; rows of block mb and half h are `in`
     int64_t first[KH];
     bool on[KH];
@@ -127,6 +124,7 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
 #pragma unroll 1
       for (int p = 0; p < kPanels; ++p) {
         NsVec<2> v[2][MB][2], m[2][MB][2];
+        float part[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -155,9 +153,11 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
                 y = make_float2(ns_update(q, y.x, n.v[0]), ns_update(q, y.y, n.v[1]));
                 if (in(mb, h) && col < q.large) ns_store<2>(q.m, base(mb, h) + col, MLPSP_PRECISION_F32, n);
               }
-              squares[h] = fmaf(y.x, y.x, fmaf(y.y, y.y, squares[h]));
+              part[h] = fmaf(y.x, y.x, fmaf(y.y, y.y, part[h]));
               keep[(p * 2 * MB * 2 + (u * MB + mb) * 2 + h) * 32] = y;
             }
+        squares[0] += part[0];
+        squares[1] += part[1];
       }
     };
     if (q.vec >= 2) {
@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
       }
     } else {
       // odd rows, transposed matrices: element by element
+      float part[2] = {0.f, 0.f};
 #pragma unroll 1
       for (int i = 0; i < kPanels * 2 * MB; ++i) {
         const int nb = i / MB, mb = i % MB;
@@ -190,8 +191,9 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
               q.m[at] = m;
             }
           }
-          squares[h] = fmaf(y[0], y[0], fmaf(y[1], y[1], squares[h]));
+          part[h] = fmaf(y[0], y[0], fmaf(y[1], y[1], part[h]));
           keep[(i * 2 + h) * 32] = make_float2(y[0], y[1]);
+          if (i % (2 * MB) == 2 * MB - 1) { squares[h] += part[h]; part[h] = 0.f; }      // panel by panel, as above
         }
       }
     }
@@ -240,6 +242,7 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
       bool again = false;
 #pragma unroll
       for (int h = 0; h < KH; ++h) {
+        if (pass == 1 && f[h] == 1.f) continue;       // settled
         start[h] = ns_start(q.eps, ss[h], f[h]);
         f[h] = start[h].lost ? kNsShrink : ss[h] < kNsTinySquares ? kNsGrow : 1.f;
         again |= f[h] != 1.f;
@@ -311,8 +314,32 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
         if (K == 2) ns_gram<MB, K, false>(hi, lo, bh, bl, d);
         else ns_gram<MB, K, false>(hi, lo, hi, lo, d);
       };
+      if (NB) {
 #pragma unroll 1
-      for (int p = 0; p < NB / 2; ++p) columns(p, NsTag<2>{});
+        for (int p = 0; p < kWhole; ++p) columns(p, NsTag<2>{});
+      } else {
+        // Long rows, four panels at a time, whose sums are added in FP32: the tensor core rounds towards zero with every MMA, and over 1,500
+        // columns that came to 6e-6 of the result
+        float sum[MB * (MB + 1)][4];
+#pragma unroll
+        for (int i = 0; i < MB * (MB + 1); ++i) sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.f;
+#pragma unroll 1
+        for (int p0 = 0; p0 < kWhole; p0 += 4) {
+#pragma unroll 1
+          for (int p = p0; p < min(p0 + 4, kWhole); ++p) columns(p, NsTag<2>{});
+#pragma unroll
+          for (int i = 0; i < MB * (MB + 1); ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              sum[i][e] += d[i][e];
+              d[i][e] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MB * (MB + 1); ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[i][e] = sum[i][e];
+      }
       if (NB & 1) columns(NB / 2, NsTag<1>{});
       NsFrag<MB> A;
       float a32[MB * (MB + 1)][4];
@@ -443,7 +470,7 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
         uint32_t hi[MB][4];
         product(0, NsTag<2>{}, e);
 #pragma unroll 1
-        for (int p = 1; p < NB / 2; ++p) {
+        for (int p = 1; p < kWhole; ++p) {
           heads(p - 1, NsTag<2>{}, hi);
           product(p, NsTag<2>{}, next);
           store(p - 1, NsTag<2>{}, e, hi);
@@ -452,9 +479,9 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
 #pragma unroll
             for (int i = 0; i < 8; ++i) e[mb][i >> 2][i & 3] = next[mb][i >> 2][i & 3];
         }
-        heads(NB / 2 - 1, NsTag<2>{}, hi);
+        heads(kWhole - 1, NsTag<2>{}, hi);
         if (NB & 1) product(NB / 2, NsTag<1>{}, next);
-        store(NB / 2 - 1, NsTag<2>{}, e, hi);
+        store(kWhole - 1, NsTag<2>{}, e, hi);
         if (NB & 1) {
           heads(NB / 2, NsTag<1>{}, hi);
           store(NB / 2, NsTag<1>{}, next, hi);
@@ -503,7 +530,7 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
         }
       };
 #pragma unroll 1
-      for (int p = 0; p < NB / 2; ++p) finish(p, NsTag<2>{});
+      for (int p = 0; p < kWhole; ++p) finish(p, NsTag<2>{});
       if (NB & 1) finish(NB / 2, NsTag<1>{});
     }
   };
@@ -513,23 +540,24 @@ __global__ void __launch_bounds__(32 * kNsWarps, CTAS * 4 / kNsWarps) k_ns_warp(
 
 template <int MB, int NB, int CTAS>
 static int ns_warp(const NsArgs& q, cudaStream_t st) {
-  constexpr int smem = kNsWarps * ns_warp_smem<MB, NB>();
-  static_assert(CTAS * 4 / kNsWarps * (smem + 1024) <= 227 * 1024, "resident CTAs");
+  constexpr int most = (NB ? (NB + 1) / 2 : kNsWarpLong[MB - 1] / 16) * ns_panel_bytes<MB>();
+  static_assert(NB == 0 || CTAS * (most + 1024) <= 227 * 1024, "resident CTAs");
+  const int smem = NB ? most : (q.large + 15) / 16 * ns_panel_bytes<MB>();
   static DeviceOnce once;
-  if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_warp<MB, NB, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_warp<MB, NB, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
   const int pack = std::max(1, 16 * MB / q.small);
-  const int64_t tiles = (q.count + pack - 1) / pack, grid = (tiles + kNsWarps - 1) / kNsWarps;
-  MLPSP_REQUIRE(grid < (1ll << 31), MLPSP_E_LIMIT, "orthogonalize: too many matrices");
+  const int64_t tiles = (q.count + pack - 1) / pack;
+  MLPSP_REQUIRE(tiles < (1ll << 31), MLPSP_E_LIMIT, "orthogonalize: too many matrices");
   const bool prefetch = reinterpret_cast<uintptr_t>(q.w) % 16 == 0 && pack * q.stride % 4 == 0;
   LaunchScope scope(kKMisc, 1, st);
-  return cuda_check(launch_chained(k_ns_warp<MB, NB, CTAS>, dim3((unsigned)grid), dim3(32 * kNsWarps), smem, st, q, pack, tiles, prefetch),
-                    "orthogonalize");
+  return cuda_check(launch_chained(k_ns_warp<MB, NB, CTAS>, dim3((unsigned)tiles), dim3(32), smem, st, q, pack, prefetch), "orthogonalize");
 }
 
 int launch_ns_warp(const NsArgs& q, cudaStream_t st) {
   const int nb = (q.large + 7) / 8;
-  if (q.small <= 16) return nb <= 4 ? ns_warp<1, 4, 8>(q, st) : nb <= 6 ? ns_warp<1, 6, 7>(q, st) : nb <= 9 ? ns_warp<1, 9, 7>(q, st) : ns_warp<1, 12, 7>(q, st);
-  return nb <= 4 ? ns_warp<2, 4, 4>(q, st) : nb <= 6 ? ns_warp<2, 6, 4>(q, st) : nb <= 9 ? ns_warp<2, 9, 4>(q, st) : ns_warp<2, 12, 4>(q, st);
+  if (nb > 12) return q.small <= 16 ? ns_warp<1, 0, 24>(q, st) : ns_warp<2, 0, 16>(q, st);
+  if (q.small <= 16) return nb <= 4 ? ns_warp<1, 4, 32>(q, st) : nb <= 6 ? ns_warp<1, 6, 28>(q, st) : nb <= 9 ? ns_warp<1, 9, 28>(q, st) : ns_warp<1, 12, 28>(q, st);
+  return nb <= 4 ? ns_warp<2, 4, 16>(q, st) : nb <= 6 ? ns_warp<2, 6, 16>(q, st) : nb <= 9 ? ns_warp<2, 9, 16>(q, st) : ns_warp<2, 12, 16>(q, st);
 }
 
 }  // namespace mlpsp

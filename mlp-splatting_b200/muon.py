@@ -43,7 +43,7 @@ def _answer(shapes, check):
     if not check or not any(L.load().mlpsp_orthogonalize_waits(rows, cols) for _n, rows, cols in shapes):
         return None
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("matrices beyond 64 x 96 wait for the kernel's answer: pass check=False inside a graph capture")
+        raise RuntimeError("matrices of these sizes wait for the kernel's answer: pass check=False inside a graph capture")
     return C.c_int32(0)
 
 
@@ -70,8 +70,9 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     update: float32, float16 or bfloat16, [rows, columns] or [N, rows, columns], contiguous; out (update itself, or a tensor
     apart from it) receives the result in update's type.  The iteration has FP32 accuracy whatever the type.  A matrix of zeros stays
     zero; one that holds an infinity or a NaN becomes NaN and touches no other.  Coefficients under which singular values leave
-    [0, 4] are refused.  Matrices beyond 64 x 96 go to a kernel with bounded waits, for whose answer the call waits
-    unless check is False."""
+    [0, 4] are refused.  Large matrices (more than 64 rows on the shorter side, or more than 512, with 33 to 64 rows 256, on the
+    longer) may go to a kernel with bounded waits, for whose answer the call waits unless check is False; where their number decides
+    on the kernel, it shows in the last bits."""
     n, rows, cols = _shape("update", update)
     if update.dtype not in _TYPES:
         raise ValueError("update must be float32, float16 or bfloat16")

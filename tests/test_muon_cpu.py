@@ -35,7 +35,7 @@ def test_c_entries_check_their_arguments():
     assert step(w=None) == -1 and step(g=None) == -1 and step(m=None) == -1
     assert step(mu=1.0) == -1 and step(mu=-0.1) == -1 and step(lr=-1.0) == -1 and step(lr=float("inf")) == -1
     assert step(wd=float("nan")) == -1 and step(scale=0.0) == -1
-    assert [lib.mlpsp_orthogonalize_waits(*s) for s in ((32, 96), (96, 32), (64, 64), (65, 65), (4, 97))] == [0, 0, 0, 1, 1]
+    assert [lib.mlpsp_orthogonalize_waits(*s) for s in ((32, 512), (512, 1), (256, 64), (65, 65), (4, 513), (33, 257))] == [0, 0, 0, 1, 1, 1]
 
 
 def test_there_is_no_cpu_path():

@@ -23,7 +23,7 @@ struct NpBlocks { float d[6][4], o[4][4]; };
 // parts PART0 on: hi lo, lo hi, hi hi
 template <int K, int PART0 = 0, int PARTS = 3>
 __device__ __forceinline__ void np_gram(uint32_t xa, uint32_t xb, int own, int off, NpBlocks& b) {
-  uint32_t ah[2][4], al[2][4], bh[2][4], bl[2][4], oh[4], ol[4];
+  uint32_t ah[2][4], al[2][4], bh[2][4], bl[2][4];
 #pragma unroll
   for (int mb = 0; mb < 2; ++mb) {
     ns_ldmatrix<K, false>(ah[mb], xa + own + mb * kNpBlock);
@@ -48,19 +48,30 @@ __device__ __forceinline__ void np_gram(uint32_t xa, uint32_t xb, int own, int o
         const auto& r = K == 2 ? (part == 0 ? bl : bh) : (part == 0 ? al : ah);
         mul(b.d[mb * (mb + 1) + n], l[mb], r[n >> 1], n & 1);
       }
+  // the block between the warps: warp 0 has its left operand already, warp 1 its right one
+  auto between = [&](const uint32_t (&th)[2][4], const uint32_t (&tl)[2][4], const uint32_t (&oh)[4], const uint32_t (&ol)[4]) {
 #pragma unroll
-  for (int mb = 0; mb < 2; ++mb) {
-    ns_ldmatrix<K, false>(ah[mb], xa + mb * kNpBlock);
-    if (PART0 < 2) ns_ldmatrix<K, false>(al[mb], xa + mb * kNpBlock + kNpLo);
+    for (int part = PART0; part < PART0 + PARTS; ++part)
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) mul(b.o[2 * mb + n], part == 1 ? tl[mb] : th[mb], part == 0 ? ol : oh, n);
+  };
+  if (own == 0) {
+    uint32_t oh[4], ol[4];
+    ns_ldmatrix<K, false>(oh, (K == 2 ? xb : xa) + off);
+    if (PART0 < 2) ns_ldmatrix<K, false>(ol, (K == 2 ? xb : xa) + off + kNpLo);
+    between(ah, al, oh, ol);
+  } else {
+    uint32_t th[2][4], tl[2][4];
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb) {
+      ns_ldmatrix<K, false>(th[mb], xa + mb * kNpBlock);
+      if (PART0 < 2) ns_ldmatrix<K, false>(tl[mb], xa + mb * kNpBlock + kNpLo);
+    }
+    if (K == 2) between(th, tl, bh[1], bl[1]);
+    else between(th, tl, ah[1], al[1]);
   }
-  ns_ldmatrix<K, false>(oh, (K == 2 ? xb : xa) + off);
-  if (PART0 < 2) ns_ldmatrix<K, false>(ol, (K == 2 ? xb : xa) + off + kNpLo);
-#pragma unroll
-  for (int part = PART0; part < PART0 + PARTS; ++part)
-#pragma unroll
-    for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) mul(b.o[2 * mb + n], part == 1 ? al[mb] : ah[mb], part == 0 ? ol : oh, n);
 }
 
 // the 16 x 16 block of a symmetric matrix at (row block i, column block j), and its transpose at (j, i)

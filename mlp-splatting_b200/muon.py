@@ -11,6 +11,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from .engine import _on, _stream_ptr
@@ -52,6 +53,11 @@ def _read(answer, what):
         raise RuntimeError(f"{what}: a device-side wait gave up; results are invalid")
 
 
+def _written(tensors):
+    """In-place writes count as such: scenes packed from the old weights are packed anew, autograd sees saved tensors change."""
+    increment_version([t for t in tensors if not t.is_inference()])
+
+
 def _coefficients(coefficients, steps, eps):
     if not isinstance(steps, int) or isinstance(steps, bool) or not 1 <= steps <= 32:
         raise ValueError("steps must be an integer from 1 to 32")
@@ -81,11 +87,14 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
         out = torch.empty_like(update, memory_format=torch.contiguous_format)
     elif out.shape != update.shape or out.dtype != update.dtype:
         raise ValueError("out must have the shape and type of update")
+    elif 0 < abs(out.data_ptr() - update.data_ptr()) < update.numel() * update.element_size():
+        raise ValueError("out must be update or lie apart from it")
     dev = _check_tensors([update, out])
     with _on(dev):
         answer = _answer([(n, rows, cols)], check)
         L.check(L.load().mlpsp_orthogonalize(L.ptr(update), _TYPES[update.dtype], n, rows, cols, *args, L.ptr(out),
                                              None if answer is None else C.byref(answer), _stream_ptr(dev)), "mlpsp_orthogonalize")
+    _written([out])
     _read(answer, "orthogonalize")
     return out
 
@@ -138,4 +147,5 @@ def muon_step(weights, grads, momenta, *, lr: float, momentum: float = 0.95, nes
             for w, g, m, (n, rows, cols) in zip(*lists, shapes)))
         L.check(lib.mlpsp_muon_step(tensors, len(shapes), L.ptr(active), lr, momentum, int(bool(nesterov)), weight_decay, *args,
                                     None if answer is None else C.byref(answer), _stream_ptr(dev)), "mlpsp_muon_step")
+    _written(lists[0] + lists[2])
     _read(answer, "muon_step")

@@ -188,6 +188,26 @@ def test_nothing_active_and_nothing_at_all():
     muon.muon_step(torch.zeros(0, 64, 72, device="cuda"), torch.zeros(0, 64, 72, device="cuda"), torch.zeros(0, 64, 72, device="cuda"), lr=1.0)
 
 
+def test_what_was_packed_from_old_weights_is_packed_anew():
+    """In-place steps count as such: the renderer's packed scene, and autograd's check of saved tensors."""
+    from mlp_splatting_b200.cumodel import NeuralPrimitiveSceneTileCUDA
+    model = NeuralPrimitiveSceneTileCUDA(num_primitives=20).cuda()
+    packed = model.packed_scene()
+    assert model.packed_scene() is packed
+    layers = [model.W1, model.W2, model.W3]
+    momenta = [torch.zeros_like(w) for w in layers]
+    saved = (model.W2 * model.W2).sum()
+    muon.muon_step(layers, [torch.randn_like(w) for w in layers], momenta, lr=0.1)
+    again = model.packed_scene()
+    assert again is not packed and torch.equal(again.W1, model.W1.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
+    out = torch.zeros(3, 4, device="cuda")
+    version = out._version
+    muon.orthogonalize(torch.ones(3, 4, device="cuda"), out=out)
+    assert out._version > version
+
+
 def test_other_streams_and_replayed_graphs():
     """A step captured on small and large matrices and replayed on new gradients; two graphs over the same tensors."""
     shapes = [(20, 32, 72), (3, 64, 64), (1, 128, 300)]
@@ -241,6 +261,7 @@ def test_refusals():
         (lambda: muon.orthogonalize(u.mT), "contiguous"),
         (lambda: muon.orthogonalize(u.cpu()), "one CUDA device"),
         (lambda: muon.orthogonalize(u, out=half), "shape and type"),
+        (lambda: muon.orthogonalize(u[:2], out=u[1:3]), "lie apart"),
         (lambda: muon.orthogonalize(u, steps=0), "steps"),
         (lambda: muon.orthogonalize(u, steps=True), "steps"),
         (lambda: muon.orthogonalize(u, eps=0.0), "eps"),

@@ -129,13 +129,17 @@ class RecordRoute:
         return int(self.slots.numel())
 
 
-def _check_route(route, *tensors):
+def _check_route(route, rows, other=None, weights=None):
+    """The calls of a small model are a dozen microseconds of host time, so these checks are written out."""
     if not isinstance(route, RecordRoute):
         raise TypeError("route must be a RecordRoute, as route_records returns it")
     slots, offsets, first = route.slots, route.offsets, route.pixel_offsets
-    for t in (slots, offsets, first, *tensors):
-        if t is not None and not (t.is_cuda and t.is_contiguous() and t.device == slots.device):
-            raise ValueError("all inputs must be contiguous tensors on one CUDA device")
+    dev = slots.get_device()
+    if (dev < 0 or offsets.get_device() != dev or rows.get_device() != dev or not slots.is_contiguous() or not offsets.is_contiguous()
+            or not rows.is_contiguous() or (first is not None and (first.get_device() != dev or not first.is_contiguous()))
+            or (other is not None and (other.get_device() != dev or not other.is_contiguous()))
+            or (weights is not None and (weights.get_device() != dev or not weights.is_contiguous()))):
+        raise ValueError("all inputs must be contiguous tensors on one CUDA device")
     if slots.dtype != torch.int32 or offsets.dtype != torch.int64 or offsets.numel() < 1:
         raise ValueError("slots must be int32 and offsets int64 with the initial zero")
     if first is None:
@@ -143,6 +147,9 @@ def _check_route(route, *tensors):
             raise ValueError("the record count must be pixels x fan")
     elif first.dtype != torch.int64 or first.ndim != 1 or first.numel() != route.pixels + 1:
         raise ValueError("pixel offsets must be int64 with one entry more than pixels")
+    if weights is not None and (weights.dtype != torch.float32 or weights.numel() != slots.numel()):
+        raise ValueError("weights must be float32, one for every record")
+    return dev
 
 
 def _check_rows(name, rows, count):
@@ -152,15 +159,23 @@ def _check_rows(name, rows, count):
         raise ValueError(f"{name} must have shape ({count}, 1..{L.ROUTE_MAX_DIM}), got {tuple(rows.shape)}")
 
 
-def _check_weights(weights, route):
-    if weights is not None and (weights.dtype != torch.float32 or weights.numel() != route.records):
-        raise ValueError("weights must be float32, one for every record")
+def _call(name, dev, *args):
+    """A row call of the library on device `dev`, whose last argument is the stream."""
+    fn = getattr(L.load(), name)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        L.check(rc, name)
 
 
 def _route_args(route):
     """(pixels, fan, pixel_offsets, slots, records, kept) of the C calls."""
-    return (route.pixels, 0 if route.pixel_offsets is not None else route.fan, L.ptr(route.pixel_offsets), L.ptr(route.slots),
-            route.records, route.offsets.data_ptr() + 8 * (route.offsets.numel() - 1))
+    first, offsets, slots = route.pixel_offsets, route.offsets, route.slots
+    return (route.pixels, route.fan if first is None else 0, None if first is None else first.data_ptr(), slots.data_ptr(), slots.numel(),
+            offsets.data_ptr() + 8 * (offsets.numel() - 1))
 
 
 def route_records(primitive_ids: torch.Tensor, num_primitives: int, pixel_offsets: torch.Tensor | None = None, *,
@@ -200,49 +215,41 @@ def route_records(primitive_ids: torch.Tensor, num_primitives: int, pixel_offset
     nbytes = int(lib.mlpsp_route_records_scratch_bytes(R, n))
     scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
     found = C.c_int32(0)
-    with _on(dev):
-        L.check(lib.mlpsp_route_records(L.ptr(ids), R, n, L.ptr(first), pixels, L.ptr(offsets), L.ptr(slots), L.ptr(scratch), nbytes,
-                                        C.byref(found) if first is not None and check else None, _stream_ptr(dev)), "mlpsp_route_records")
+    _call("mlpsp_route_records", ids.get_device(), ids.data_ptr(), R, n, L.ptr(first), pixels, offsets.data_ptr(), slots.data_ptr(),
+          L.ptr(scratch), nbytes, C.byref(found) if first is not None and check else None)
     if found.value & L.ROUTE_BAD_OFFSETS:
         raise ValueError("pixel offsets must start at zero, end at the record count and be monotone")
     return RecordRoute(offsets, slots, pixels, fan, first)
 
 
 def _dispatch(x, route):
-    _check_route(route, x)
+    dev = _check_route(route, x)
     _check_rows("x", x, route.pixels)
-    out = torch.empty((route.records, x.shape[1]), device=x.device, dtype=x.dtype)
-    with _on(x.device):
-        L.check(L.load().mlpsp_dispatch_rows(L.ptr(x), _ROW_TYPES[x.dtype], x.shape[1], *_route_args(route), L.ptr(out),
-                                             _stream_ptr(x.device)), "mlpsp_dispatch_rows")
+    out = x.new_empty((route.slots.numel(), x.shape[1]))
+    _call("mlpsp_dispatch_rows", dev, x.data_ptr(), _ROW_TYPES[x.dtype], x.shape[1], *_route_args(route), out.data_ptr())
     return out
 
 
 def _combine(y, route, weights, name="y"):
-    _check_route(route, y, weights)
-    _check_rows(name, y, route.records)
-    _check_weights(weights, route)
-    out = torch.empty((route.pixels, y.shape[1]), device=y.device, dtype=y.dtype)
-    with _on(y.device):
-        L.check(L.load().mlpsp_combine_rows(L.ptr(y), _ROW_TYPES[y.dtype], y.shape[1], L.ptr(weights), *_route_args(route), L.ptr(out),
-                                            _stream_ptr(y.device)), "mlpsp_combine_rows")
+    dev = _check_route(route, y, None, weights)
+    _check_rows(name, y, route.slots.numel())
+    out = y.new_empty((route.pixels, y.shape[1]))
+    _call("mlpsp_combine_rows", dev, y.data_ptr(), _ROW_TYPES[y.dtype], y.shape[1], None if weights is None else weights.data_ptr(),
+          *_route_args(route), out.data_ptr())
     return out
 
 
 def _combine_gradients(grad_out, y, route, weights, want_y, want_weights):
-    _check_route(route, grad_out, y, weights)
+    dev = _check_route(route, grad_out, y, weights)
     _check_rows("grad_out", grad_out, route.pixels)
-    _check_rows("y", y, route.records)
+    _check_rows("y", y, route.slots.numel())
     if y.dtype != grad_out.dtype or y.shape[1] != grad_out.shape[1]:
         raise ValueError("grad_out and y must have one element type and row length")
-    _check_weights(weights, route)
     grad_y = torch.empty_like(y) if want_y else None
     grad_weights = torch.empty_like(weights) if want_weights else None
     if want_y or want_weights:
-        with _on(y.device):
-            L.check(L.load().mlpsp_combine_rows_gradients(
-                L.ptr(grad_out), L.ptr(y), _ROW_TYPES[y.dtype], y.shape[1], L.ptr(weights), *_route_args(route), L.ptr(grad_y),
-                L.ptr(grad_weights), _stream_ptr(y.device)), "mlpsp_combine_rows_gradients")
+        _call("mlpsp_combine_rows_gradients", dev, grad_out.data_ptr(), y.data_ptr(), _ROW_TYPES[y.dtype], y.shape[1], L.ptr(weights),
+              *_route_args(route), L.ptr(grad_y), L.ptr(grad_weights))
     return grad_y, grad_weights
 
 

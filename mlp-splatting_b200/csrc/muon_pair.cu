@@ -14,7 +14,7 @@
 namespace mlpsp {
 
 constexpr int kNpThreads = 64, kNpRows = 64, kNpPanel = kNpRows * 64, kNpLo = kNpPanel / 2, kNpBlock = 16 * 32;
-__host__ __device__ constexpr int np_smem(int panels) { return (panels + 4) * kNpPanel + 32; }
+__host__ __device__ constexpr int np_smem(int panels) { return (panels + 4) * kNpPanel + 32 + 4 * kNpRows; }
 
 // d: blocks (mb, n), n <= 2 mb + 1, of the warp's own rows at mb (mb + 1) + n; o: blocks (mb, n) of rows 16 mb, columns 32 + 16 w + 8 n at 2 mb + n
 struct NpBlocks { float d[6][4], o[4][4]; };
@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
   const uint32_t xb = xs + ((lane & 7) + ((lane >> 4) << 3)) * 32 + ((((lane >> 3) & 1) ^ ((lane >> 2) & 1)) << 4);
   const uint32_t aa = xa + kPanels * kNpPanel, ab = xb + kPanels * kNpPanel;      // A's panels behind X's
   float* const s_sum = reinterpret_cast<float*>(smem + (kPanels + 4) * kNpPanel);   // [2][2] sums of squares, by pass and warp
+  float* const s_diag = s_sum + 8;                                                   // [64] the diagonal of A
   // this lane's values of a panel in FP32, [2 columns of blocks][2 blocks of rows][2], in the places of its rows' heads and tails
   auto keep = [&](int p, int u, int mb, int h) -> float2& {
     return *reinterpret_cast<float2*>(smem + p * kNpPanel + u * kNpLo + own + ((mb * 2 + h) * 32 + lane) * 8);
@@ -276,9 +277,18 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
 #pragma unroll
         for (int i = 0; i < 4; ++i) A.o[i][e] *= by.gram;
       }
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float (&b)[4] = A.d[mb * (mb + 1) + 2 * mb + h];       // the block on the diagonal: lane 4 g + g / 2 has row g's element
+          if (t == g >> 1) s_diag[32 * w + mb * 16 + h * 8 + g] = g & 1 ? b[2 * h + 1] : b[2 * h];
+          if (2 * t == g) b[2 * h] = 0.f;
+          if (2 * t + 1 == g) b[2 * h + 1] = 0.f;
+        }
       np_put(aa, w, A);
       __syncthreads();
-      // ---- P = b A + c A^2 but for its diagonal, which is kept apart (muon_warp.cu)
+      // ---- P = b A + c A^2, diagonals apart (muon_warp.cu)
 #pragma unroll
       for (int i = 0; i < 6; ++i) S.d[i][0] = S.d[i][1] = S.d[i][2] = S.d[i][3] = 0.f;
 #pragma unroll
@@ -287,20 +297,30 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
       for (int p = 0; p < 4; ++p) np_gram<2, 0, 2>(aa + p * kNpPanel, ab + p * kNpPanel, own, off, S);
 #pragma unroll 1
       for (int p = 0; p < 4; ++p) np_gram<2, 2, 1>(aa + p * kNpPanel, ab + p * kNpPanel, own, off, S);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-#pragma unroll
-        for (int i = 0; i < 6; ++i) S.d[i][e] = fmaf(by.b, A.d[i][e], by.c * S.d[i][e]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) S.o[i][e] = fmaf(by.b, A.o[i][e], by.c * S.o[i][e]);
-      }
       float diag[2][2];        // a + P(r, r) of this lane's rows
+      auto form = [&](float (&o)[4], const float (&e)[4], int row0, int col0) {
+        const float2 c = *reinterpret_cast<const float2*>(s_diag + col0 + 2 * t);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float row_of = fmaf(by.c, s_diag[row0 + h * 8 + g], by.b);
+          o[2 * h] = fmaf(by.c, o[2 * h], e[2 * h] * fmaf(by.c, c.x, row_of));
+          o[2 * h + 1] = fmaf(by.c, o[2 * h + 1], e[2 * h + 1] * fmaf(by.c, c.y, row_of));
+        }
+      };
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) {
+#pragma unroll
+        for (int n = 0; n < 2 * mb + 2; ++n) form(S.d[mb * (mb + 1) + n], A.d[mb * (mb + 1) + n], 32 * w + 16 * mb, 32 * w + 8 * n);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) form(S.o[2 * mb + n], A.o[2 * mb + n], 16 * mb, 32 + 16 * w + 8 * n);
+      }
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float (&b)[4] = S.d[mb * (mb + 1) + 2 * mb + h];       // the block on the diagonal: lane 4 g + g / 2 has row g's element
-          diag[mb][h] = by.a + __shfl_sync(0xffffffffu, g & 1 ? b[2 * h + 1] : b[2 * h], 4 * g + (g >> 1));
+          float (&b)[4] = S.d[mb * (mb + 1) + 2 * mb + h];
+          const float d = s_diag[32 * w + mb * 16 + h * 8 + g];
+          diag[mb][h] = fmaf(d, fmaf(by.c, d, by.b), by.a) + __shfl_sync(0xffffffffu, g & 1 ? b[2 * h + 1] : b[2 * h], 4 * g + (g >> 1));
           if (2 * t == g) b[2 * h] = 0.f;
           if (2 * t + 1 == g) b[2 * h + 1] = 0.f;
         }

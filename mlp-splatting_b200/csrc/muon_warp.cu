@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(32, CTAS) k_ns_warp(const NsArgs q, const int 
       }
       if (NB & 1) columns(NB / 2, NsTag<1>{});
       NsFrag<MB> A;
-      float a32[MB * (MB + 1)][4];
+      float a32[MB * (MB + 1)][4], diag[MB][2];       // diag: of this lane's rows
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -356,12 +356,23 @@ __global__ void __launch_bounds__(32, CTAS) k_ns_warp(const NsArgs q, const int 
               if (MB == 1 && !(same >> (h * 4 + n * 2 + e) & 1u)) v = 0.f;
               a32[i][2 * h + e] = v;
             }
+            if (n == 2 * mb + h) {       // the block on the diagonal: lane 4 g + g / 2 has row g's element
+              diag[mb][h] = __shfl_sync(0xffffffffu, g & 1 ? a32[i][2 * h + 1] : a32[i][2 * h], 4 * g + (g >> 1));
+              if (2 * t == g) a32[i][2 * h] = 0.f;
+              if (2 * t + 1 == g) a32[i][2 * h + 1] = 0.f;
+            }
             ns_split2(a32[i][2 * h], a32[i][2 * h + 1], A.hi[mb][n][h], A.lo[mb][n][h]);
           }
       ns_mirror<MB>(A);
       float own[MB][2];        // a + P(r, r) of this lane's rows
-      // ---- P = b A + c A^2.  Its diagonal is kept apart and multiplies X in FP32 below: the rest is smaller, and with it what the tensor
-      // core's rounding towards zero takes off (4e-6 of the result for 128 rows with the diagonal in, 2e-6 so)
+      float across[2 * MB][2]; // D of this lane's columns
+#pragma unroll
+      for (int n = 0; n < 2 * MB; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) across[n][e] = __shfl_sync(0xffffffffu, diag[n >> 1][n & 1], 4 * (2 * t + e));
+      // ---- P = b A + c A^2, diagonals apart: with A = D + E, A^2 = D^2 + D E + E D + E^2, of which the tensor core forms E^2, and P's
+      // diagonal multiplies X in FP32 below.  What is left to the tensor core is smaller, and with it what 22 bits and rounding towards zero take
+      // off: 0.9 of a plain FP32 iteration's error instead of 1.3 for matrices of 4 x 32, half of 4e-6 for 128 rows.
 #pragma unroll
       for (int round = 0; round < 2; ++round)
 #pragma unroll
@@ -388,9 +399,11 @@ __global__ void __launch_bounds__(32, CTAS) k_ns_warp(const NsArgs q, const int 
           for (int h = 0; h < 2; ++h) {
             const int i = mb * (mb + 1) + n;
             const NsStep& s = by[h % KH];
-            float v0 = fmaf(s.b, a32[i][2 * h], s.c * d[i][2 * h]), v1 = fmaf(s.b, a32[i][2 * h + 1], s.c * d[i][2 * h + 1]);
-            if (n == 2 * mb + h) {       // the block on the diagonal: lane 4 g + g / 2 has row g's element
-              own[mb][h] = s.a + __shfl_sync(0xffffffffu, g & 1 ? v1 : v0, 4 * g + (g >> 1));
+            const float row_of = fmaf(s.c, diag[mb][h], s.b);
+            float v0 = fmaf(s.c, d[i][2 * h], a32[i][2 * h] * fmaf(s.c, across[n][0], row_of));
+            float v1 = fmaf(s.c, d[i][2 * h + 1], a32[i][2 * h + 1] * fmaf(s.c, across[n][1], row_of));
+            if (n == 2 * mb + h) {
+              own[mb][h] = fmaf(diag[mb][h], row_of, s.a) + __shfl_sync(0xffffffffu, g & 1 ? v1 : v0, 4 * g + (g >> 1));
               if (2 * t == g) v0 = 0.f;
               if (2 * t + 1 == g) v1 = 0.f;
             }

@@ -9,10 +9,9 @@
 // when there is more than one digit, for the offsets, which are found by binary search inside the range of their highest digit.
 // Up to 65,536 records of up to 511 primitives take one launch of a cluster of eight CTAs.
 //
-// Bound: latency of the ranking (sixteen warps a CTA, three CTAs per SM; passes of six bits at two CTAs of eight warps took 95 us each for
-// 7.8 M records) and, in the last pass of several, the scattered words.  7.8 M records of 100,000 primitives: 330 -> 177 us (59 and 74 of
-// them the placements); 32,764 of
-// 256: 35 -> 10 us.
+// Bound: latency of the ranking (sixteen warps a CTA, three CTAs per SM; passes of six bits with sixteen warps per SM took 95 us each for
+// 7.8 M records) and, in the last pass of several, the scattered words.  7.8 M records of 100,000 primitives: 330 -> 177 us, of which the
+// placements take 59 and 74; 32,764 of 256: 35 -> 10 us.
 #include "frame.cuh"
 
 namespace mlpsp {

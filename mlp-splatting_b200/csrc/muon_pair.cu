@@ -8,7 +8,7 @@
 //
 // A tcgen05 tile holds two such matrices at a time and spends half of its products on the blocks between them: with the passes through
 // tensor memory a 64 x 72 matrix took 97 ns of the GPU that way, 57 here (five steps, thousands of matrices), where mma.sync is busy for 70
-// percent of the time.  As in muon_warp.cu small products come before large ones.
+// percent of the time and shared memory for as much.
 #include "muon_mma.cuh"
 
 namespace mlpsp {
@@ -20,17 +20,16 @@ __host__ __device__ constexpr int np_smem(int panels) { return (panels + 4) * kN
 struct NpBlocks { float d[6][4], o[4][4]; };
 
 // += x x^T over a panel of 8 K columns at `at`; own, top, off: byte offsets of the warp's rows, of row 0 and of row 32 + 16 w
-// parts PART0 on: hi lo, lo hi, hi hi
-template <int K, int PART0 = 0, int PARTS = 3>
+template <int K>
 __device__ __forceinline__ void np_gram(uint32_t xa, uint32_t xb, int own, int off, NpBlocks& b) {
   uint32_t ah[2][4], al[2][4], bh[2][4], bl[2][4];
 #pragma unroll
   for (int mb = 0; mb < 2; ++mb) {
     ns_ldmatrix<K, false>(ah[mb], xa + own + mb * kNpBlock);
-    if (PART0 < 2) ns_ldmatrix<K, false>(al[mb], xa + own + mb * kNpBlock + kNpLo);
+    ns_ldmatrix<K, false>(al[mb], xa + own + mb * kNpBlock + kNpLo);
     if (K == 2) {
       ns_ldmatrix<K, false>(bh[mb], xb + own + mb * kNpBlock);
-      if (PART0 < 2) ns_ldmatrix<K, false>(bl[mb], xb + own + mb * kNpBlock + kNpLo);
+      ns_ldmatrix<K, false>(bl[mb], xb + own + mb * kNpBlock + kNpLo);
     }
   }
   // word of rows 8 h of a block as the B operand's first or second
@@ -39,7 +38,7 @@ __device__ __forceinline__ void np_gram(uint32_t xa, uint32_t xb, int own, int o
     else ns_mma8(d, l[0], l[1], r[h]);
   };
 #pragma unroll
-  for (int part = PART0; part < PART0 + PARTS; ++part)
+  for (int part = 0; part < 3; ++part)
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -51,7 +50,7 @@ __device__ __forceinline__ void np_gram(uint32_t xa, uint32_t xb, int own, int o
   // the block between the warps: warp 0 has its left operand already, warp 1 its right one
   auto between = [&](const uint32_t (&th)[2][4], const uint32_t (&tl)[2][4], const uint32_t (&oh)[4], const uint32_t (&ol)[4]) {
 #pragma unroll
-    for (int part = PART0; part < PART0 + PARTS; ++part)
+    for (int part = 0; part < 3; ++part)
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -60,14 +59,14 @@ __device__ __forceinline__ void np_gram(uint32_t xa, uint32_t xb, int own, int o
   if (own == 0) {
     uint32_t oh[4], ol[4];
     ns_ldmatrix<K, false>(oh, (K == 2 ? xb : xa) + off);
-    if (PART0 < 2) ns_ldmatrix<K, false>(ol, (K == 2 ? xb : xa) + off + kNpLo);
+    ns_ldmatrix<K, false>(ol, (K == 2 ? xb : xa) + off + kNpLo);
     between(ah, al, oh, ol);
   } else {
     uint32_t th[2][4], tl[2][4];
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb) {
       ns_ldmatrix<K, false>(th[mb], xa + mb * kNpBlock);
-      if (PART0 < 2) ns_ldmatrix<K, false>(tl[mb], xa + mb * kNpBlock + kNpLo);
+      ns_ldmatrix<K, false>(tl[mb], xa + mb * kNpBlock + kNpLo);
     }
     if (K == 2) between(th, tl, bh[1], bl[1]);
     else between(th, tl, ah[1], al[1]);
@@ -294,9 +293,7 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
 #pragma unroll
       for (int i = 0; i < 4; ++i) S.o[i][0] = S.o[i][1] = S.o[i][2] = S.o[i][3] = 0.f;
 #pragma unroll 1
-      for (int p = 0; p < 4; ++p) np_gram<2, 0, 2>(aa + p * kNpPanel, ab + p * kNpPanel, own, off, S);
-#pragma unroll 1
-      for (int p = 0; p < 4; ++p) np_gram<2, 2, 1>(aa + p * kNpPanel, ab + p * kNpPanel, own, off, S);
+      for (int p = 0; p < 4; ++p) np_gram<2>(aa + p * kNpPanel, ab + p * kNpPanel, own, off, S);
       float diag[2][2];        // a + P(r, r) of this lane's rows
       auto form = [&](float (&o)[4], const float (&e)[4], int row0, int col0) {
         const float2 c = *reinterpret_cast<const float2*>(s_diag + col0 + 2 * t);

@@ -85,12 +85,15 @@ __global__ void __launch_bounds__(kRtThreads) k_dispatch(const typename RtPiece<
   }
 }
 
-// CTAS: at least so many CTAs per SM.  Six, which caps the registers at 40, suit rows of several FP32 pieces, whose lines come from all over
-// memory (730,000 rows of 512 bytes 93 -> 80 us); one-piece rows (35 -> 42 us) and 16-bit ones, with twice the sums (7 -> 11), do not.
+// CTAS: at least so many CTAs per SM.  Six make the compiler spill (40 registers instead of 48), which costs where y comes from the L2 and
+// pays where it comes from memory in FP32 rows of at least 64 bytes, by the rows that are then on their way: 49,000 and 730,000 rows of 512 bytes
+// (25 and 374 MB) 5.4 -> 8.2 and 93 -> 80 us, 1.4 M of 64 bytes (90 MB) 33 -> 30; of 48 (67 MB) 20 -> 25, 7.5 M of 16 45 -> 48.  The
+// 16-bit types, with twice the sums, lose everywhere.
+constexpr int64_t kRtFromMemory = 80ll << 20;
 template <typename T, int B, int CTAS>
-__global__ void __launch_bounds__(kRtThreads, CTAS) k_combine(const typename RtPiece<B>::type* __restrict__ y, const float* __restrict__ weights,
-                                                        RouteView v, int pieces, int cb, int ppb,
-                                                        typename RtPiece<B>::type* __restrict__ out) {
+__global__ void __launch_bounds__(kRtThreads, CTAS) k_combine(const typename RtPiece<B>::type* __restrict__ y,
+                                                              const float* __restrict__ weights, RouteView v, int pieces, int cb,
+                                                              int ppb, typename RtPiece<B>::type* __restrict__ out) {
   chain_wait();
   chain_release();
   using V = typename RtPiece<B>::type;
@@ -261,8 +264,11 @@ template <typename T, int B>
 static void combine_rows(const void* y, const float* weights, const RouteView& v, int64_t row_bytes, void* out, cudaStream_t st) {
   using V = typename RtPiece<B>::type;
   const RtShape s = rt_shape(row_bytes, B, v.pixels);
-  constexpr int most = sizeof(T) == 4 ? 6 : 1;
-  launch_chained(s.pieces > 1 ? k_combine<T, B, most> : k_combine<T, B, 1>, s.grid, s.block, 0, st, static_cast<const V*>(y), weights, v, s.pieces, s.cb, s.ppb, static_cast<V*>(out));
+  auto* kernel = k_combine<T, B, 1>;
+  if constexpr (sizeof(T) == 4 && B == 16)
+    if (row_bytes >= 64 && v.records * row_bytes >= kRtFromMemory) kernel = k_combine<T, B, 6>;
+  launch_chained(kernel, s.grid, s.block, 0, st, static_cast<const V*>(y), weights, v,
+                 s.pieces, s.cb, s.ppb, static_cast<V*>(out));
 }
 
 template <typename T, int B>
@@ -273,8 +279,9 @@ static void combine_grad(const void* dout, const void* y, const float* weights, 
   int lanes = 1;
   while (lanes < 32 && lanes < pieces) lanes *= 2;
   const int ppb = (int)std::min<int64_t>(kRtPixels, std::max<int64_t>(1, v.pixels / (sm_count() * 8)));      // eight blocks per SM, if pixels last
-  launch_chained(pieces >= 8 && pieces <= 64 ? k_combine_grad<T, B, 4> : k_combine_grad<T, B, 2>, dim3((unsigned)((v.pixels + ppb - 1) / ppb)), dim3(kRtThreads), 0, st, static_cast<const V*>(dout),
-                 static_cast<const V*>(y), weights, v, pieces, lanes, ppb, static_cast<V*>(dy), dw);
+  launch_chained(pieces >= 8 && pieces <= 64 ? k_combine_grad<T, B, 4> : k_combine_grad<T, B, 2>,
+                 dim3((unsigned)((v.pixels + ppb - 1) / ppb)), dim3(kRtThreads), 0, st, static_cast<const V*>(dout), static_cast<const V*>(y),
+                 weights, v, pieces, lanes, ppb, static_cast<V*>(dy), dw);
 }
 
 }  // namespace mlpsp

@@ -58,7 +58,7 @@ __device__ __forceinline__ void nt_get(const char* hi, const char* lo, float (&x
 }
 
 // `np` columns per CTA, `pack` matrices per tile
-__global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const int np, const int cluster, const int pack, const int64_t tiles) {
+__global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const int np, const int cluster, const int pack) {
   ns_begin(q);
   extern __shared__ __align__(1024) char smem[];
   const int tid = threadIdx.x, warp = warp_of_cta();
@@ -127,11 +127,11 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
     }
   };
 
-  for (int64_t tile = blockIdx.x / cluster; tile < tiles; tile += gridDim.x / cluster) {
-    const int64_t k = tile * pack + sub;
+  auto work = [&] {
+    const int64_t k = (int64_t)(blockIdx.x / cluster) * pack + sub;
     const bool in = sub < pack && k < q.count && (!q.active || q.active[k]);
     const int64_t base = in ? k * q.stride + (int64_t)srow * q.rs : 0;
-    if (!__syncthreads_or(in)) continue;         // the same answer in every CTA of a cluster: they hold slices of the same matrices
+    if (!__syncthreads_or(in)) return;         // the same answer in every CTA of a cluster: they hold slices of the same matrices
     // ---- momentum, and the update's values in FP32 in the places of X's pairs (eight to a pair of 16-byte words); sums of squares
     float4 ss = make_float4(0.f, 0.f, 0.f, 0.f);
     auto load = [&](auto width) {
@@ -428,7 +428,8 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
       s_xsq[part * kNtRows + row] = xsq;
       ready();
     }
-  }
+  };
+  work();
   if (!ok && q.gave_up) *q.gave_up = 1;
   __syncthreads();
   if (warp == 0) tmem_free(tmem, kNtTmemCols);
@@ -436,22 +437,31 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
   ns_end(q);
 }
 
-// CTAs that share a matrix: slices of 64 to 128 columns (to 256 beyond 1,024), since the exchange costs as much as the products it spreads
-static int nt_cluster(int large) { return std::min(kNtMaxCluster, std::max(1, (large + 127) / 128)); }
+// CTAs that share a matrix.  With few matrices slices of about 128 columns, since the exchange costs as much as the products it spreads; with
+// more than fit the GPU at once, and up to 256 columns, as few CTAs as hold a matrix: one of 128 x 512 70 us in four and 85 in two, forty
+// 141 and 88; one of 128 x 144 59 us in two and 49 in one.  (Seven eighths of the SMs: clusters of eight leave the odd ones of a GPC.)
+static int nt_cluster(const NsArgs& q) {
+  const int64_t pack = kNtRows / q.small, tiles = (q.count + pack - 1) / pack;
+  const int narrow = std::min(kNtMaxCluster, (q.large + 127) / 128), wide = (q.large + kNtMaxCols - 1) / kNtMaxCols;
+  return wide > 1 && tiles * narrow <= sm_count() * 7 / 8 ? narrow : wide;
+}
 // whether the tiles need more than two rounds of all clusters
-static bool ns_many(const NsArgs& q) { return (q.count + kNtRows / q.small - 1) / (kNtRows / q.small) > 2 * (int64_t)(sm_count() / nt_cluster(q.large)); }
+static bool ns_many(const NsArgs& q) {
+  const int64_t pack = kNtRows / q.small;
+  return (q.count + pack - 1) / pack > 2 * (int64_t)(sm_count() / ((q.large + kNtMaxCols - 1) / kNtMaxCols));
+}
 
 int launch_ns_cluster(const NsArgs& q, cudaStream_t st) {
-  const int cluster = nt_cluster(q.large);
+  const int cluster = nt_cluster(q);
   const int np = ((q.large + cluster - 1) / cluster + 15) / 16 * 16;
   const int pack = kNtRows / q.small;
   const int64_t tiles = (q.count + pack - 1) / pack;
   const int smem = nt_smem(np);
   static DeviceOnce once;
   if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, nt_smem(kNtMaxCols)));
-  const int64_t most = std::max<int64_t>(1, (int64_t)sm_count() / cluster);
+  MLPSP_REQUIRE(tiles * cluster < (1ll << 31), MLPSP_E_LIMIT, "orthogonalize: too many matrices");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(std::min(tiles, most) * cluster));
+  cfg.gridDim = dim3((unsigned)(tiles * cluster));
   cfg.blockDim = dim3(kNtThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -464,7 +474,7 @@ int launch_ns_cluster(const NsArgs& q, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   LaunchScope scope(kKMisc, 1, st);
-  return cuda_check(cudaLaunchKernelEx(&cfg, k_ns_cluster, q, np, cluster, pack, tiles), "orthogonalize");
+  return cuda_check(cudaLaunchKernelEx(&cfg, k_ns_cluster, q, np, cluster, pack), "orthogonalize");
 }
 
 // Whether the iteration stays in the binary16 range of the scaled operands: from singular values in [0, 1], values within [-4, 4] and

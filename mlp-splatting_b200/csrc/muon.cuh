@@ -1,12 +1,13 @@
-// What the two Newton-Schulz kernels share: arguments, element access, the split of an FP32 value into two binary16 ones.
+// What the three Newton-Schulz kernels share: arguments, element access, the split of an FP32 value into two binary16 ones.
 //
 //   X0 = U / max(|U|_F, eps),   X <- a X + (b A + c A^2) X,  A = X X^T   (X the matrix or its transpose, whichever is wider)
 //
 // Arithmetic: the iteration multiplies a small singular value by up to a^steps (485 with the usual coefficients), so operands of
 // eleven bits would put errors of tenths into an orthogonal matrix.  X, A and bA + cA^2 are held as binary16 pairs hi + lo
 // (22 bits; X and A, whose entries become small, scaled by 2^10, so that their absolute error stays below 3e-11), every product is
-// hi hi + hi lo + lo hi on the tensor cores with FP32 accumulation, and a X is added in FP32.  On Gaussian matrices the result
-// is then 1e-6 off 64-bit arithmetic, as near as an FP32 iteration comes (1.1e-6).
+// hi hi + hi lo + lo hi on the tensor cores with FP32 accumulation, and a X is added in FP32, with the diagonals of A, A^2 and P.  On
+// Gaussian matrices the result is then nearer to 64-bit arithmetic than an iteration in plain FP32: 8e-7 and 9.5e-7 (32 x 72), 7e-7 and
+// 1e-6 (64 x 72), 1.1e-6 and 2.5e-6 (128 x 1152).
 #pragma once
 #include <type_traits>
 #include "frame.cuh"
@@ -155,12 +156,13 @@ __device__ __forceinline__ void ns_end(const NsArgs& q) {
 }
 
 // Which kernel: a warp for matrices of up to 32 rows (muon_warp.cu), two for up to 64 (muon_pair.cu), a CTA or a cluster for the rest
-// (muon_tc.cu).  Up to kNsFew columns the first two are as fast with a single matrix and faster with many; beyond, a cluster is done sooner
-// with few but its 128 rows are mostly empty, so they take over once the clusters would go round more than twice, as far as a warp's or
-// pair's X fits an SM's shared memory.
+// (muon_tc.cu).  Up to kNsWarpFew or kNsPairFew columns the first two are as fast with a single matrix and much faster with many.  Beyond, a cluster is done sooner
+// with few, though its 128 rows are mostly empty (one of 32 x 700 106 us in a warp, 70 in a cluster; of 64 x 300 79 and 62), and behind that
+// with many while enough of a warp's or pair's X fit an SM's shared memory: 2,000 of 32 x 700 877 and 974, of 64 x 350 700 and 1,136, but
+// of 64 x 400 1,522 and 1,035, 3,000 of 32 x 1,024 3,586 and 2,013.  Many: more than the clusters take at once (200 of 64 x 264 75 and 129).
 constexpr int kNsWarpRows = 32, kNsPairRows = 64;
 constexpr int kNsWarpFew = 512, kNsPairFew = 256;
-constexpr int kNsWarpLong[2] = {2048, 1024}, kNsPairLong = 512;       // warp: up to 16 rows, up to 32
+constexpr int kNsWarpLong[2] = {1024, 800}, kNsPairLong = 384;       // warp: up to 16 rows, up to 32
 int launch_ns_warp(const NsArgs& q, cudaStream_t st);
 int launch_ns_pair(const NsArgs& q, cudaStream_t st);
 int launch_ns_cluster(const NsArgs& q, cudaStream_t st);

@@ -1,4 +1,4 @@
-// Newton-Schulz iteration of matrices up to 128 x 2048 on the 5th-generation tensor cores (tcgen05), and the C entries of both kernels.
+// Newton-Schulz iteration of matrices up to 128 x 2048 on the 5th-generation tensor cores (tcgen05), and the C entries.
 //
 // A CTA holds a slice of X, 128 rows by up to 256 columns, in shared memory as binary16 pairs, in chunks of [128 rows][8 columns].
 // The same bytes are the K-major operands of A = X X^T and, read MN-major, the B operand of (bA + cA^2) X.  A matrix of more columns
@@ -438,17 +438,19 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
 }
 
 // CTAs that share a matrix.  With few matrices slices of about 128 columns, since the exchange costs as much as the products it spreads; with
-// more than fit the GPU at once, and up to 256 columns, as few CTAs as hold a matrix: one of 128 x 512 70 us in four and 85 in two, forty
-// 141 and 88; one of 128 x 144 59 us in two and 49 in one.  (Seven eighths of the SMs: clusters of eight leave the odd ones of a GPC.)
+// more than fit the GPU at once, and up to 256 columns, as few CTAs as hold a matrix: one of 128 x 512 66 us in four and 81 in two, forty
+// 137 and 84; one of 128 x 144 56 us in two and 45 in one.  (Four fifths of the SMs: clusters of eight leave the odd ones of a GPC, fewer than
+// sixteen fit; sixteen of 128 x 1152 152 us in eight CTAs each, eighteen 93 in five.)  A cluster per tile, not a loop over tiles in as many
+// clusters as there are SMs for: those that did not fit waited for a whole loop, 400 of 128 x 2048 4,182 us instead of 2,529.
 static int nt_cluster(const NsArgs& q) {
   const int64_t pack = kNtRows / q.small, tiles = (q.count + pack - 1) / pack;
   const int narrow = std::min(kNtMaxCluster, (q.large + 127) / 128), wide = (q.large + kNtMaxCols - 1) / kNtMaxCols;
-  return wide > 1 && tiles * narrow <= sm_count() * 7 / 8 ? narrow : wide;
+  return wide > 1 && tiles * narrow <= sm_count() * 4 / 5 ? narrow : wide;
 }
-// whether the tiles need more than two rounds of all clusters
+// whether there are more tiles than clusters on the GPU
 static bool ns_many(const NsArgs& q) {
   const int64_t pack = kNtRows / q.small;
-  return (q.count + pack - 1) / pack > 2 * (int64_t)(sm_count() / ((q.large + kNtMaxCols - 1) / kNtMaxCols));
+  return (q.count + pack - 1) / pack * ((q.large + kNtMaxCols - 1) / kNtMaxCols) > sm_count();
 }
 
 int launch_ns_cluster(const NsArgs& q, cudaStream_t st) {

@@ -66,8 +66,7 @@ __device__ __forceinline__ void ns_prefetch(const void* p, int64_t i, int n, int
 
 // One tile per warp: which tiles an SM takes is left to the hardware.  With as many CTAs as fit the GPU walking the tiles in turn, the
 // slowest SM set the time and its warps fell into step, all loading and then all multiplying: a step of 100,000 matrices of 32 x 72
-// 2,540 us, now 1,720 (of which 704 are its bytes).  prefetch: a tile's weights, wanted last, are brought into L2 when it starts (1,817
-// without).  Twenty warps per SM instead of sixteen: 2,160.
+// 2,540 us, so 1,750 (of which 704 are its bytes).  prefetch: a tile's weights, wanted last, are brought into L2 when it starts (5 percent).  Twenty warps per SM instead of sixteen: 2,160.
 template <int MB, int NB, int CTAS>
 __global__ void __launch_bounds__(32, CTAS) k_ns_warp(const NsArgs q, const int pack, const bool prefetch) {
   constexpr int KH = MB == 1 ? 2 : 1;       // with one block of rows, rows h = 0 and 1 of a lane may belong to two matrices

@@ -66,6 +66,30 @@ def test_iteration(n, r, c, dtype):
     assert float((one.cpu().double() - want[0]).norm()) <= tol
 
 
+# more matrices than the GPU takes at once, at the borders between the kernels and between their splits of a matrix
+MANY = [(1300, 5, 700), (1200, 16, 1000), (1200, 16, 1024), (320, 1030, 16), (700, 32, 800), (700, 32, 801), (400, 64, 384), (300, 64, 385), (250, 40, 300),
+        (60, 128, 700), (40, 97, 1500), (20, 128, 2048), (150, 128, 256), (160, 128, 257), (3, 128, 256), (3, 70, 144), (2, 1300, 90)]
+
+
+@pytest.mark.parametrize("n,r,c", MANY)
+def test_many_long_matrices(n, r, c):
+    u = stack(n, r, c, seed=n + r + c)
+    want, tol = allowed(u)
+    out = muon.orthogonalize(u.cuda())
+    assert float((out.cpu().double() - want).norm()) <= tol
+    # an inactive matrix and its neighbours
+    active = torch.arange(n) % 5 != 2
+    w, m = stack(n, r, c, seed=1).cuda(), torch.zeros(n, r, c, device="cuda")
+    before = w.clone()
+    muon.muon_step(w, u.cuda(), m, lr=1.0, momentum=0.0, active=active.cuda())
+    assert torch.equal(w[~active], before[~active]) and not m[~active].any()
+    # w - scale X, with an FP32 rounding of the product and of the difference each
+    scale = math.sqrt(max(1.0, r / c))
+    step = before.cpu().double() - scale * want
+    tol = scale * tol + 2.0 ** -23 * (float(before.double().norm()) + 2 * scale * float(want.norm()))
+    assert float((w.cpu().double() - step)[active].norm()) <= tol
+
+
 @pytest.mark.parametrize("how", [dict(steps=1), dict(steps=12), dict(coefficients=(1.5, -0.5, 0.0), steps=9),
                                  dict(coefficients=(1.875, -1.25, 0.375), steps=7), dict(eps=1.0, steps=3)])
 @pytest.mark.parametrize("n,r,c", [(9, 32, 72), (5, 4, 32), (3, 64, 72), (1, 128, 300)])

@@ -161,26 +161,30 @@ __global__ void __launch_bounds__(kRtThreads) k_combine_grad(const typename RtPi
   const uint32_t kept = rt_kept(v), all = (uint32_t)v.records;
   const int sub = threadIdx.x & (lanes - 1), groups = kRtThreads / lanes;
   const uint32_t group = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
-  for (int64_t r0 = first + threadIdx.x / lanes; r0 < last; r0 += (int64_t)groups * U) {
+  for (int64_t r0 = first + (int64_t)(threadIdx.x / lanes) * U; r0 < last; r0 += (int64_t)groups * U) {
     uint32_t s[U];
     float w[U], dot[U];
     size_t pixel[U];
+    int lo = 0;
+    if (v.pixel_offsets) {         // the last of the block's pixels whose first record is not behind r0
+      int hi = here;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_first[mid] <= r0) lo = mid; else hi = mid;
+      }
+    } else {
+      lo = (int)(r0 - first) / v.fan;
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t r = r0 + u * groups;
+      const int64_t r = r0 + u;
       const bool valid = r < last;
       s[u] = valid ? (uint32_t)__ldg(v.slots + r) : 0xffffffffu;
       w[u] = valid && weights ? __ldg(weights + r) : 1.f;
       dot[u] = 0.f;
-      int lo = 0;
-      if (v.pixel_offsets) {       // the last of the block's pixels whose first record is not behind r
-        int hi = here;
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (s_first[mid] <= r) lo = mid; else hi = mid;
-        }
-      } else if (valid) {
-        lo = (int)(r - first) / v.fan;
+      if (u > 0 && valid) {
+        if (v.pixel_offsets) while (lo + 1 < here && s_first[lo + 1] <= r) ++lo;
+        else lo += (lo + 1) * (int64_t)v.fan <= r - first;
       }
       pixel[u] = (size_t)(p0 + lo);
     }
@@ -219,7 +223,7 @@ __global__ void __launch_bounds__(kRtThreads) k_combine_grad(const typename RtPi
       if (sub == 0)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (r0 + u * groups < last) dw[r0 + u * groups] = dot[u];
+          if (r0 + u < last) dw[r0 + u] = dot[u];
     }
   }
 }

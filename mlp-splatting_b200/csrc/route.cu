@@ -133,11 +133,12 @@ __global__ void __launch_bounds__(kRtThreads, CTAS) k_combine(const typename RtP
   out[(size_t)p * pieces + c] = o;
 }
 
-// Every record for itself: `lanes` (a power of two) neighbouring threads take one, U records a time whose rows are then on their way together.
-// A block has the records of `ppb` pixels, so slots, weights and dw are read and written in order; the pixel of a record is found by binary
-// search among the block's offsets.  4.6 M records of 16-byte rows: 121 us with a thread per pixel (its dw words lie in 32 sectors), 69 so.
-// U is four for rows that fill a group of eight lanes or more (950,000 rows of 128 bytes 90 us, by twos 98; of 66 bytes in 2-byte pieces 152
-// and 188), else two (16-byte rows 69 us, by fours 77; 16,000 rows of 4,096 bytes, several rounds of a warp, 35 and 45).
+// Every record for itself: `lanes` (a power of two) neighbouring threads take U consecutive ones a time, whose rows are then on their way
+// together.  A block has the records of `ppb` pixels, so slots, weights and dw are read and written in order; the pixel of the first record is
+// found by binary search among the block's offsets, those of the others by steps from there.  4.6 M records of 16-byte rows: 121 us with a
+// thread per pixel (its dw words lie in 32 sectors), 66 so; 950,000 of 128 bytes 90 with a search for each, 73 so.
+// U is four for rows of two to 64 pieces (combine and gradients of 950,000 rows of 128 bytes 107 us, by twos 127; of 475,000 of 66 bytes in
+// 2-byte pieces 155 and 208), else two (76,000 of 16 bytes, too few for all SMs, 10 us, by fours 13; 16,000 of 4,096 43 and 47).
 constexpr int kRtPixels = 256;
 template <typename T, int B, int U>
 __global__ void __launch_bounds__(kRtThreads) k_combine_grad(const typename RtPiece<B>::type* __restrict__ dout,
@@ -283,7 +284,7 @@ static void combine_grad(const void* dout, const void* y, const float* weights, 
   int lanes = 1;
   while (lanes < 32 && lanes < pieces) lanes *= 2;
   const int ppb = (int)std::min<int64_t>(kRtPixels, std::max<int64_t>(1, v.pixels / (sm_count() * 8)));      // eight blocks per SM, if pixels last
-  launch_chained(pieces >= 8 && pieces <= 64 ? k_combine_grad<T, B, 4> : k_combine_grad<T, B, 2>,
+  launch_chained(pieces >= 2 && pieces <= 64 ? k_combine_grad<T, B, 4> : k_combine_grad<T, B, 2>,
                  dim3((unsigned)((v.pixels + ppb - 1) / ppb)), dim3(kRtThreads), 0, st, static_cast<const V*>(dout), static_cast<const V*>(y),
                  weights, v, pieces, lanes, ppb, static_cast<V*>(dy), dw);
 }

@@ -307,3 +307,23 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="singular values leave"):
         muon.orthogonalize(u, coefficients=(5.0, 1.0, 1.0))
     assert bool((u == 1).all())
+
+
+@pytest.mark.parametrize("n,r,c", [(932_100, 32, 72), (4_200_000, 16, 32), (524_400, 64, 64), (131_200, 128, 128)])
+def test_stacks_beyond_32_bits(n, r, c):
+    """More than 2^31 elements: the last matrices come out as they do alone, in place."""
+    u = torch.empty(n, r, c, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(n))
+    assert u.numel() > 2 ** 31
+    tail, head = u[-8:].clone(), u[:8].clone()
+    assert muon.orthogonalize(u, out=u) is u
+    assert torch.equal(u[-8:], muon.orthogonalize(tail)) and torch.equal(u[:8], muon.orthogonalize(head))
+
+
+def test_a_step_beyond_32_bits():
+    n, r, c = 932_100, 32, 72
+    g = torch.empty(n, r, c, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(3))
+    w, m = torch.ones(n, r, c, device="cuda"), torch.zeros(n, r, c, device="cuda")
+    last = [t[-5:].clone() for t in (w, g, m)]
+    muon.muon_step(w, g, m, lr=0.1)
+    muon.muon_step(*last, lr=0.1)
+    assert torch.equal(w[-5:], last[0]) and torch.equal(m[-5:], last[2])

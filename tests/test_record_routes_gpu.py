@@ -275,3 +275,33 @@ def test_route_at_the_borders_of_its_passes(N, R):
     route = pc.route_records(ids.to(torch.int32).cuda(), N)
     offsets, slots = plain_route(ids, N)
     assert torch.equal(route.offsets.cpu(), offsets) and torch.equal(route.slots.cpu().long(), slots)
+
+
+@pytest.mark.parametrize("R", [1, 5000, 70_000])
+def test_no_primitives_at_all(R):
+    route = pc.route_records(torch.zeros(R, 1, dtype=torch.int32, device="cuda"), 0)
+    assert route.offsets.tolist() == [0] and torch.equal(route.slots.cpu().long(), torch.arange(R))
+    x = torch.ones(R, 3, device="cuda")
+    assert not pc.dispatch_rows(x, route).any() and not pc.combine_rows(x * float("nan"), route).any()
+
+
+def test_rows_beyond_32_bits():
+    """2^31 elements and more on both sides; a permutation of rows and its way back."""
+    T, D, N = 33_000, 65_536, 500
+    ids = torch.randint(0, N, (T, 1), generator=torch.Generator().manual_seed(1), dtype=torch.int32).cuda()
+    route = pc.route_records(ids, N)
+    x = torch.empty(T, D, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(2))
+    assert x.numel() > 2 ** 31
+    rows = pc.dispatch_rows(x, route)
+    slots = route.slots.long()
+    for at in (0, T // 2, T - 2, T - 1):
+        assert torch.equal(rows[slots[at]], x[at])
+    back = pc.combine_rows(rows, route)
+    assert torch.equal(back, x)
+    del back
+    two = torch.full((T, 1), 2.0, device="cuda")
+    grad, grad_w = pc.combine_rows_gradients(x, rows, route, two)
+    assert torch.equal(grad[slots[T - 1]], 2 * x[T - 1]) and torch.equal(grad[slots[0]], 2 * x[0])
+    # <x, x> of 65,536 squares, each sum of products off by at most 2^-24 of the terms so far per step, in at most 2^12 steps
+    for at in (0, T - 1):
+        assert abs(float(grad_w[at, 0]) - float(x[at].double().square().sum())) <= 2.0 ** -12 * D * 2

@@ -1,11 +1,14 @@
 """The training operators together, on the records of a rendered image: routing, evaluation, compositing as a weighted sum, its gradients,
 weight gradients, and a step on the weights."""
 import math
+import threading
 
 import numpy as np
 import pytest
 import torch
 
+from mlp_splatting_b200 import muon
+from mlp_splatting_b200 import primitive_csr as pc
 from tests.helpers import WKEYS, oracle_frame, small_case
 
 pytestmark = pytest.mark.gpu
@@ -79,3 +82,40 @@ def test_a_step_from_records_to_weights():
         seen = direction.flatten(1).norm(dim=1) > 0
         size = torch.linalg.matrix_norm(moved[seen], ord=2)
         assert bool((size < 1.3).all()) and bool((size > 0.3).all())      # singular values towards one
+
+
+def test_calls_of_two_threads():
+    """Each on its own stream, with calls that wait for an answer: neither sees the other's."""
+    def work(seed, out):
+        g = torch.Generator().manual_seed(seed)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(20):
+                first = torch.tensor([0, 900, 2_000, 70_000 + i])
+                ids = torch.randint(-1, 700, (70_000 + i,), generator=g, dtype=torch.int32)
+                if (seed + i) % 3 == 0:
+                    first[1] = 80_000
+                u = torch.randn(2, 128, 300, generator=g)
+                w, m = torch.randn(5, 64, 400, generator=g).cuda(), torch.zeros(5, 64, 400, device="cuda")
+                grads = torch.randn(5, 64, 400, generator=g).cuda()
+                try:
+                    route = pc.route_records(ids.cuda(), 700, first.cuda())
+                    x = torch.randn(3, 65, generator=g).cuda()
+                    out.append(pc.combine_rows(pc.dispatch_rows(x, route), route).cpu())
+                    out.append(route.slots.cpu())
+                except ValueError as e:
+                    out.append(str(e))
+                out.append(muon.orthogonalize(u.cuda()).cpu())
+                muon.muon_step(w, grads, m, lr=0.1)
+                out.append(w.cpu())
+
+    want, got = [[], []], [[], []]
+    for k in range(2):
+        work(k, want[k])
+    threads = [threading.Thread(target=work, args=(k, got[k])) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(want[0] + want[1], got[0] + got[1]):
+        assert a == b if isinstance(a, str) else torch.equal(a, b)
+    assert [len(a) for a in want] == [len(b) for b in got] and any(isinstance(a, str) for a in want[0])

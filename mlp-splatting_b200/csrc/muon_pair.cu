@@ -7,8 +7,8 @@
 // writes its rows of them back.
 //
 // A tcgen05 tile holds two such matrices at a time and spends half of its products on the blocks between them: with the passes through
-// tensor memory a 64 x 72 matrix took 97 ns of the GPU that way, 57 here (five steps, thousands of matrices), where mma.sync is busy for 70
-// percent of the time and shared memory for as much.
+// tensor memory a 64 x 72 matrix took 97 ns of the GPU that way, 57 here (five steps, thousands of matrices), where mma.sync is busy for 55
+// percent of the time and shared memory for 60 to 70.
 #include "muon_mma.cuh"
 
 namespace mlpsp {

@@ -11,7 +11,7 @@
 // launch looks like, in FP32, and rounded once; no atomics.  Bound: memory, one visit of every record's row.
 //
 // Rows move in pieces of up to 16 bytes (the widest that the row length and all addresses are a multiple of).  dispatch and combine
-// give a thread one piece of one pixel: neighbouring threads take neighbouring pieces, so the lines of a row are whole whatever its
+// give a thread one piece of one pixel, or two where pieces are small: neighbouring threads take neighbouring pieces, so the lines of a row are whole whatever its
 // length, and a short row does not idle lanes.
 #include "frame.cuh"
 #include <cuda_bf16.h>
@@ -53,15 +53,16 @@ template <> __device__ __forceinline__ float rt_round<float>(float x) { return x
 template <> __device__ __forceinline__ __half rt_round<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 rt_round<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// the pixel and the piece of this thread: `ppb` pixels of `cb` pieces each per block, blocks of pieces along y
+// the pixel and the first piece of this thread, of K that lie cb apart: `ppb` pixels of `cb` threads each per block, blocks of pieces along y
+template <int K>
 __device__ __forceinline__ bool rt_place(int pieces, int cb, int ppb, int64_t pixels, int64_t& p, int& c) {
   const int local = threadIdx.x / cb;
   p = (int64_t)blockIdx.x * ppb + local;
-  c = blockIdx.y * cb + (threadIdx.x - local * cb);
+  c = blockIdx.y * cb * K + (threadIdx.x - local * cb);
   return local < ppb && p < pixels && c < pieces;
 }
 
-template <int B>
+template <int B, int K>
 __global__ void __launch_bounds__(kRtThreads) k_dispatch(const typename RtPiece<B>::type* __restrict__ x, RouteView v, int pieces,
                                                          int cb, int ppb, typename RtPiece<B>::type* __restrict__ out) {
   chain_wait();
@@ -69,11 +70,14 @@ __global__ void __launch_bounds__(kRtThreads) k_dispatch(const typename RtPiece<
   using V = typename RtPiece<B>::type;
   int64_t p, b, e;
   int c;
-  if (!rt_place(pieces, cb, ppb, v.pixels, p, c)) return;
+  if (!rt_place<K>(pieces, cb, ppb, v.pixels, p, c)) return;
   rt_range(v, p, b, e);
   if (b >= e) return;
   const uint32_t kept = rt_kept(v), all = (uint32_t)v.records;
-  const V row = __ldg(x + (size_t)p * pieces + c);
+  V row[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (c + k * cb < pieces) row[k] = __ldg(x + (size_t)p * pieces + c + k * cb);
   const V zero = {};
   for (int64_t r = b; r < e; r += 4) {
     uint32_t s[4];
@@ -81,7 +85,9 @@ __global__ void __launch_bounds__(kRtThreads) k_dispatch(const typename RtPiece<
     for (int u = 0; u < 4; ++u) s[u] = r + u < e ? (uint32_t)__ldg(v.slots + r + u) : all;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (s[u] < all) out[(size_t)s[u] * pieces + c] = s[u] < kept ? row : zero;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (s[u] < all && c + k * cb < pieces) out[(size_t)s[u] * pieces + c + k * cb] = s[u] < kept ? row[k] : zero;
   }
 }
 
@@ -90,7 +96,7 @@ __global__ void __launch_bounds__(kRtThreads) k_dispatch(const typename RtPiece<
 // (25 and 374 MB) 5.4 -> 8.2 and 93 -> 80 us, 1.4 M of 64 bytes (90 MB) 33 -> 30; of 48 (67 MB) 20 -> 25, 7.5 M of 16 45 -> 48.  The
 // 16-bit types, with twice the sums, lose everywhere.
 constexpr int64_t kRtFromMemory = 80ll << 20;
-template <typename T, int B, int CTAS>
+template <typename T, int B, int K, int CTAS>
 __global__ void __launch_bounds__(kRtThreads, CTAS) k_combine(const typename RtPiece<B>::type* __restrict__ y,
                                                               const float* __restrict__ weights, RouteView v, int pieces, int cb,
                                                               int ppb, typename RtPiece<B>::type* __restrict__ out) {
@@ -100,16 +106,18 @@ __global__ void __launch_bounds__(kRtThreads, CTAS) k_combine(const typename RtP
   constexpr int E = B / (int)sizeof(T);
   int64_t p, b, e;
   int c;
-  if (!rt_place(pieces, cb, ppb, v.pixels, p, c)) return;
+  if (!rt_place<K>(pieces, cb, ppb, v.pixels, p, c)) return;
   rt_range(v, p, b, e);
   const uint32_t kept = rt_kept(v);
-  float acc[E];
+  float acc[K][E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) acc[i] = 0.f;
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[k][i] = 0.f;
   for (int64_t r = b; r < e; r += 4) {
     uint32_t s[4];
     float w[4];
-    V row[4];
+    V row[4][K];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       s[u] = r + u < e ? (uint32_t)__ldg(v.slots + r + u) : 0xffffffffu;
@@ -117,26 +125,37 @@ __global__ void __launch_bounds__(kRtThreads, CTAS) k_combine(const typename RtP
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (s[u] < kept) row[u] = __ldg(y + (size_t)s[u] * pieces + c);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (s[u] < kept && c + k * cb < pieces) row[u][k] = __ldg(y + (size_t)s[u] * pieces + c + k * cb);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (s[u] < kept) {
-        const T* f = reinterpret_cast<const T*>(&row[u]);
 #pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] = fmaf(w[u], rt_float(f[i]), acc[i]);
-      }
+      for (int k = 0; k < K; ++k)
+        if (s[u] < kept && c + k * cb < pieces) {
+          const T* f = reinterpret_cast<const T*>(&row[u][k]);
+#pragma unroll
+          for (int i = 0; i < E; ++i) acc[k][i] = fmaf(w[u], rt_float(f[i]), acc[k][i]);
+        }
   }
-  V o;
-  T* f = reinterpret_cast<T*>(&o);
 #pragma unroll
-  for (int i = 0; i < E; ++i) f[i] = rt_round<T>(acc[i]);
-  out[(size_t)p * pieces + c] = o;
+  for (int k = 0; k < K; ++k)
+    if (c + k * cb < pieces) {
+      V o;
+      T* f = reinterpret_cast<T*>(&o);
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = rt_round<T>(acc[k][i]);
+      out[(size_t)p * pieces + c + k * cb] = o;
+    }
 }
 
 // Every record for itself: `lanes` (a power of two) neighbouring threads take U consecutive ones a time, whose rows are then on their way
 // together.  A block has the records of `ppb` pixels, so slots, weights and dw are read and written in order; the pixel of the first record is
-// found by binary search among the block's offsets, those of the others by steps from there.  4.6 M records of 16-byte rows: 121 us with a
-// thread per pixel (its dw words lie in 32 sectors), 66 so; 950,000 of 128 bytes 90 with a search for each, 73 so.
+// found by binary search among the block's offsets, those of the others by steps from there.  A group has about as many lanes as rounds: what
+// every lane does once a record (slot, weight, sum over the lanes) and idle lanes of the last round cost more than short runs of a row: 570,000
+// rows of 256 bytes in four lanes 56 us, in eight 62, in sixteen 67, in two 68; 475,000 of 33 bf16 values in eight 54, in 32 112.  4.6 M records of 16-byte rows: 121 us with a
+// thread per pixel (its dw words lie in 32 sectors), 66 so; 950,000 of 128 bytes 90 with a search for each, 73
+// with one for four.
 // U is four for rows of two to 64 pieces (combine and gradients of 950,000 rows of 128 bytes 107 us, by twos 127; of 475,000 of 66 bytes in
 // 2-byte pieces 155 and 208), else two (76,000 of 16 bytes, too few for all SMs, 10 us, by fours 13; 16,000 of 4,096 43 and 47).
 constexpr int kRtPixels = 256;
@@ -247,13 +266,16 @@ static int rt_check(const char* who, const RouteView& v, int64_t dim, int32_t dt
   return MLPSP_OK;
 }
 
+// whether so many threads fill the GPU; else each has one piece (2,850 rows of 33 bf16 values: gradients 3.4 us, with the rules for many 5.1)
+static bool rt_fills(int64_t threads) { return threads >= (int64_t)sm_count() * 1024; }
+
 struct RtShape { int pieces, cb, ppb; dim3 grid, block; };
-static RtShape rt_shape(int64_t row_bytes, int piece, int64_t pixels) {
+static RtShape rt_shape(int64_t row_bytes, int piece, int k, int64_t pixels) {
   RtShape s;
   s.pieces = (int)(row_bytes / piece);
-  s.cb = std::min(s.pieces, kRtThreads);
+  s.cb = std::min((s.pieces + k - 1) / k, kRtThreads);
   s.ppb = kRtThreads / s.cb;
-  s.grid = dim3((unsigned)((pixels + s.ppb - 1) / s.ppb), (unsigned)((s.pieces + s.cb - 1) / s.cb));
+  s.grid = dim3((unsigned)((pixels + s.ppb - 1) / s.ppb), (unsigned)((s.pieces + s.cb * k - 1) / (s.cb * k)));
   s.block = dim3((unsigned)((s.ppb * s.cb + 31) / 32 * 32));
   return s;
 }
@@ -261,17 +283,29 @@ static RtShape rt_shape(int64_t row_bytes, int piece, int64_t pixels) {
 template <int B>
 static void dispatch_rows(const void* x, const RouteView& v, int64_t row_bytes, void* out, cudaStream_t st) {
   using V = typename RtPiece<B>::type;
-  const RtShape s = rt_shape(row_bytes, B, v.pixels);
-  launch_chained(k_dispatch<B>, s.grid, s.block, 0, st, static_cast<const V*>(x), v, s.pieces, s.cb, s.ppb, static_cast<V*>(out));
+  // Two pieces a thread where they are small and many, to share the slots: 190,000 rows of 33 FP32 values 25 -> 21 us, 38,000 of 513 bf16 ones
+  // 26 -> 20, but 2 M of 7 FP32 24.6 -> 26, 2.8 M of 3 fp16 26 -> 39, 475,000 of 34 FP32 in 8-byte pieces 15 -> 18.
+  const int k = B <= 4 && row_bytes / B >= 12 && rt_fills(v.pixels * (row_bytes / B) / 2) ? 2 : 1;
+  const RtShape s = rt_shape(row_bytes, B, k, v.pixels);
+  auto* kernel = k_dispatch<B, 1>;
+  if constexpr (B <= 4)
+    if (k == 2) kernel = k_dispatch<B, 2>;
+  launch_chained(kernel, s.grid, s.block, 0, st, static_cast<const V*>(x), v, s.pieces, s.cb, s.ppb, static_cast<V*>(out));
 }
 
 template <typename T, int B>
 static void combine_rows(const void* y, const float* weights, const RouteView& v, int64_t row_bytes, void* out, cudaStream_t st) {
   using V = typename RtPiece<B>::type;
-  const RtShape s = rt_shape(row_bytes, B, v.pixels);
-  auto* kernel = k_combine<T, B, 1>;
+  // Two pieces a thread where they are one or two values, to share slots and weights: 475,000 rows of 33 FP32 values 32 -> 24 us, 2.8 M of 13 bf16
+  // 138 -> 95, 57,000 of 530 29 -> 24, but 2.8 M of 6 bf16 21 -> 23.5, 1.9 M of 12 fp16 (in pieces of four) 18 -> 22.
+  constexpr bool few = B / (int)sizeof(T) <= 2;
+  const int k = few && row_bytes / B >= 4 && rt_fills(v.pixels * (row_bytes / B) / 2) ? 2 : 1;
+  const RtShape s = rt_shape(row_bytes, B, k, v.pixels);
+  auto* kernel = k_combine<T, B, 1, 1>;
+  if constexpr (few)
+    if (k == 2) kernel = k_combine<T, B, 2, 1>;
   if constexpr (sizeof(T) == 4 && B == 16)
-    if (row_bytes >= 64 && v.records * row_bytes >= kRtFromMemory) kernel = k_combine<T, B, 6>;
+    if (row_bytes >= 64 && v.records * row_bytes >= kRtFromMemory) kernel = k_combine<T, B, 1, 6>;
   launch_chained(kernel, s.grid, s.block, 0, st, static_cast<const V*>(y), weights, v,
                  s.pieces, s.cb, s.ppb, static_cast<V*>(out));
 }
@@ -281,8 +315,9 @@ static void combine_grad(const void* dout, const void* y, const float* weights, 
                          float* dw, cudaStream_t st) {
   using V = typename RtPiece<B>::type;
   const int pieces = (int)(row_bytes / B);
+  const bool long_row = B == 16 && pieces >= 64;       // 1 KB and more: a warp (78,000 rows of 1 KB 52 us, in eight lanes 58)
   int lanes = 1;
-  while (lanes < 32 && lanes < pieces) lanes *= 2;
+  while (lanes < 32 && lanes < pieces && (lanes * lanes < pieces || long_row || !rt_fills(v.records * lanes))) lanes *= 2;
   const int ppb = (int)std::min<int64_t>(kRtPixels, std::max<int64_t>(1, v.pixels / (sm_count() * 8)));      // eight blocks per SM, if pixels last
   launch_chained(pieces >= 2 && pieces <= 64 ? k_combine_grad<T, B, 4> : k_combine_grad<T, B, 2>,
                  dim3((unsigned)((v.pixels + ppb - 1) / ppb)), dim3(kRtThreads), 0, st, static_cast<const V*>(dout), static_cast<const V*>(y),

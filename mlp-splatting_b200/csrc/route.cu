@@ -11,8 +11,8 @@
 // launch looks like, in FP32, and rounded once; no atomics.  Bound: memory, one visit of every record's row.
 //
 // Rows move in pieces of up to 16 bytes (the widest that the row length and all addresses are a multiple of).  dispatch and combine
-// give a thread one piece of one pixel, or two where pieces are small: neighbouring threads take neighbouring pieces, so the lines of a row are whole whatever its
-// length, and a short row does not idle lanes.
+// give a thread one piece of one pixel, or two where pieces are small: neighbouring threads take neighbouring pieces, so the lines of a
+// row are whole whatever its length, and a short row does not idle lanes.  dw is a sum over lanes, whose number is a choice for speed.
 #include "frame.cuh"
 #include <cuda_bf16.h>
 

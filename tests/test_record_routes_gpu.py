@@ -108,6 +108,14 @@ def test_rows_there_and_back(T, N, fan, D, dtype):
     assert pc.combine_rows_gradients(dout.cuda(), y_dev.cuda(), route)[1] is None
 
 
+@pytest.mark.parametrize("T,N,fan,D,dtype", [(30_000, 300, 0, D, t) for D in (6, 13, 33) for t in DTYPES]
+                         + [(4_000, 70, 3, D, t) for D in (130, 513) for t in DTYPES]
+                         + [(45_000, 300, 0, 128, torch.float32), (20_000, 9, 4, 260, torch.float16), (9_000, 400, 0, 256, torch.bfloat16)])
+def test_many_rows_there_and_back(T, N, fan, D, dtype):
+    """Enough of them for the kernels' other shapes: threads with two pieces, narrow groups, y beyond the L2."""
+    test_rows_there_and_back(T, N, fan, D, dtype)
+
+
 @pytest.mark.parametrize("fan", [3, 0])
 def test_autograd_is_the_gradient(fan):
     """Through autograd, with an expanded gradient, against the same program in 64 bits; and against differences."""

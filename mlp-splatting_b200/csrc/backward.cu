@@ -729,9 +729,7 @@ static int run_vjp_plan(const mlpsp_scene* sc, const float* x6, const float* d4,
                                          out, partial, st);
     if (rc) return rc;
   } else if (max_items > 0) {
-    static DeviceOnce attr_once;
-    if (attr_once.first())
-      MLPSP_CUDA_OK(cudaFuncSetAttribute(k_grouped_vjp, cudaFuncAttributeMaxDynamicSharedMemorySize, kGradSmem));
+    MLPSP_SHARED_MEMORY(kGradSmem, (const void*)k_grouped_vjp);
     const int vec = ((reinterpret_cast<uintptr_t>(sc->W1) | reinterpret_cast<uintptr_t>(sc->W2)) & 15) == 0;
     launch_chained(k_grouped_vjp, dim3((unsigned)std::min<int64_t>(max_items, (int64_t)sm_count() * kGfCtas)), dim3(kGfThreads), kGradSmem, st,
                    x6, d4, masks, items, max_items, counters, sc->freq, sc->att, sc->W1, sc->b1, sc->W2, sc->b2, sc->W3, vec, loss_scale, out, partial);
@@ -818,9 +816,7 @@ extern "C" int mlpsp_records_reverse_checked(const int32_t* ids, const int64_t* 
                  pixels, bad, findings_host ? hw.word : nullptr);
   if (findings_host) MLPSP_CUDA_OK(cudaEventRecord(ev, st));
   if (pixels > 0 && total_records > 0) {
-    static DeviceOnce attr_once;
-    if (attr_once.first())
-      MLPSP_CUDA_OK(cudaFuncSetAttribute(k_reverse_geometry, cudaFuncAttributeMaxDynamicSharedMemorySize, kRevSmem));
+    MLPSP_SHARED_MEMORY(kRevSmem, (const void*)k_reverse_geometry);
     launch_chained(k_reverse_pixels, dim3((unsigned)((pixels + kRevPixels - 1) / kRevPixels)), dim3(kRevPixels), 0, st, offsets, raw, grad_rgb, grad_t, pixels, d4, kw, bad);
     launch_chained(k_reverse_geometry, dim3((unsigned)((total_records + kRevChunk - 1) / kRevChunk)), dim3(kRevThreads),
                    kRevSmem, st, ids, x6, kw, quats,

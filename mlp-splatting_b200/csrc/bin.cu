@@ -569,16 +569,9 @@ static int bin_camera(const mlpsp_frame* fr, bool matrices, BinCam& cam) {
 }
 
 static int corner_shared_memory() {
-  static DeviceOnce attr_once;
-  if (!attr_once.first()) return MLPSP_OK;
-  auto allow = [](const void* kernel) {
-    return cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024), "bin");
-  };
   constexpr int N = kViewsPerLaunch;
-  const void* kernels[4] = {(const void*)k_bin_offsets<1>, (const void*)k_bin_offsets<N>, (const void*)k_bin_corners<true, 1>,
-                            (const void*)k_bin_corners<true, N>};
-  for (const void* k : kernels)
-    if (const int rc = allow(k)) return rc;
+  MLPSP_SHARED_MEMORY(200 * 1024, (const void*)k_bin_offsets<1>, (const void*)k_bin_offsets<N>, (const void*)k_bin_corners<true, 1>,
+                      (const void*)k_bin_corners<true, N>);
   return MLPSP_OK;
 }
 

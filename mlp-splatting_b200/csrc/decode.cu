@@ -688,10 +688,7 @@ extern "C" int mlpsp_pack_decoder(const mlpsp_decoder* dec, int32_t mode, void* 
   if (mode == 1) {
     folded = reinterpret_cast<float*>((char*)packed + h.total_bytes);
     fb = folded + (size_t)dec->num_classes * dec->hidden;
-    static DeviceOnce fold_once;
-    if (fold_once.first()) {
-      MLPSP_CUDA_OK(cudaFuncSetAttribute(k_fold_text, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-    }
+    MLPSP_SHARED_MEMORY(160 * 1024, (const void*)k_fold_text);
     k_fold_text<<<dec->num_classes, 128, dec->out_dim * 4, st>>>(dec->text, dec->W3, dec->b3, dec->out_dim, dec->hidden, folded, fb);
   }
   k_pack_decoder<<<64, 256, 0, st>>>(h, dec->W1, dec->b1, dec->W2, dec->b2, dec->W3, dec->b3, folded, fb, (char*)packed, status);
@@ -710,10 +707,7 @@ extern "C" int mlpsp_decode_features(const mlpsp_decoder* dec, int32_t mode, con
   MLPSP_REQUIRE((reinterpret_cast<uintptr_t>(packed) & 15) == 0 && (reinterpret_cast<uintptr_t>(feat) & 15) == 0 &&
                 (mode == 1 || (reinterpret_cast<uintptr_t>(out) & 15) == 0), MLPSP_E_ARG,
                 "mlpsp_decode_features: buffers must be 16-byte aligned");
-  static DeviceOnce decode_once;
-  if (decode_once.first()) {
-    MLPSP_CUDA_OK(cudaFuncSetAttribute(k_decode_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmem));
-  }
+  MLPSP_SHARED_MEMORY(kDecSmem, (const void*)k_decode_tc);
   const int sms = sm_count();
   const int tiles_x = (width + kDecTileW - 1) / kDecTileW, tiles_y = (height + kDecTileH - 1) / kDecTileH;
   const int num_tiles = tiles_x * tiles_y;

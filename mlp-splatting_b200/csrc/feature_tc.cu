@@ -336,9 +336,7 @@ template <int S, int PR>
 static int launch_ft(const mlpsp_scene* sc, const mlpsp_frame* fr, const Scratch& s, const uint32_t* used32, int T, int ntx, int CB,
                      cudaStream_t st) {
   const int smem = FtPlan<S, PR>::smem_bytes(CB);
-  static DeviceOnce attr_once;
-  if (attr_once.first())
-    MLPSP_CUDA_OK(cudaFuncSetAttribute(k_feature_tc<S, PR>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024));
+  MLPSP_SHARED_MEMORY(113 * 1024, (const void*)k_feature_tc<S, PR>);
   const dim3 grid(T, sc->feat_dim / CB);
   k_feature_tc<S, PR><<<grid, kFtThreads, smem, st>>>(fr->tile_offsets, s.tile_len, fr->sorted_prims, fr->width, fr->height, ntx, used32,
                                                       s.masks32, s.pair_base, s.rec_w, s.rec_gate, (const __half*)sc->feat16, sc->feat_dim, CB,

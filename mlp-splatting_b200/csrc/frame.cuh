@@ -3,8 +3,10 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstdarg>
+#include <initializer_list>
 #include <utility>
 #include "common.cuh"
+#include "device_once.h"
 
 namespace mlpsp {
 
@@ -197,19 +199,22 @@ int cuda_check(cudaError_t e, const char* what);
 // SMs of the current device (asked once per device)
 int sm_count();
 
-// Per-device "first use" marker for settings that CUDA keeps per device (the opt-in dynamic shared-memory
-// size of a kernel, for one): a process that drives several GPUs must apply them once on each.  The caller
-// keeps one DeviceOnce per setting; first() answers true the first time it is asked with a given device current.
-struct DeviceOnce {
-  bool seen[64] = {false};
-  bool first() {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return true;   // unknown device: apply every time
-    if (seen[dev]) return false;
-    seen[dev] = true;
-    return true;
-  }
-};
+// lets kernels use up to `bytes` of dynamic shared memory on the current device
+inline int allow_shared_memory(DeviceOnce& once, int bytes, std::initializer_list<const void*> kernels) {
+  int device = -1;
+  if (cudaGetDevice(&device) != cudaSuccess) device = -1;
+  return once.apply(device, [&] {
+    for (const void* k : kernels)
+      if (const int rc = cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute")) return rc;
+    return 0;
+  });
+}
+#define MLPSP_SHARED_MEMORY(bytes, ...)                                                          \
+  do {                                                                                           \
+    static ::mlpsp::DeviceOnce once__;                                                           \
+    const int rc__ = ::mlpsp::allow_shared_memory(once__, (int)(bytes), {__VA_ARGS__});          \
+    if (rc__ != 0) return rc__;                                                                  \
+  } while (0)
 
 // A few words of page-locked host memory that kernels write directly, and an event to wait for the kernel that does so:
 // a finding reaches the host without a copy, and without waiting for whatever was launched behind it.  One per host

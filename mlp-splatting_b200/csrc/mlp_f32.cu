@@ -538,9 +538,7 @@ int launch_mlp_f32(const mlpsp_scene* sc, const RecIn* rec_in, const int4* work,
   }
   if (F == kTF && H == 64 && !rec_ext) {
     using N = WideNet;
-    static DeviceOnce attr_once;
-    if (attr_once.first())
-      MLPSP_CUDA_OK(cudaFuncSetAttribute(k_mlp_f32_wide, cudaFuncAttributeMaxDynamicSharedMemorySize, N::kFloats * 4));
+    MLPSP_SHARED_MEMORY(N::kFloats * 4, (const void*)k_mlp_f32_wide);
     const int want = sms * N::kCtas;
     return cuda_check(launch_chained(k_mlp_f32_wide, dim3(grid_cap > 0 ? std::min(grid_cap, want) : want), dim3(N::kThreads), N::kFloats * 4, st,
                                      sc->W1, sc->b1, sc->W2, sc->b2, sc->W3, sc->b3, sc->freq, sc->att, rec_in, work, ctr, rec_out, out_mode, status),

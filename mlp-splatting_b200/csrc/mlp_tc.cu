@@ -967,9 +967,7 @@ template <bool KEEP, bool BF16, int H, bool TAB>
 static int launch_one(const char* image, const mlpsp_scene* sc, const char* dir_table, const RecIn* rec_in, const int4* work,
                       const int32_t* counters, float4* rec_out, float4* rec_ext, int out_mode, int32_t* status, cudaStream_t st, int grid) {
   using N = Net<H>;
-  static DeviceOnce attr_once;
-  if (attr_once.first())
-    MLPSP_CUDA_OK(cudaFuncSetAttribute(k_mlp_tc<KEEP, BF16, H, TAB>, cudaFuncAttributeMaxDynamicSharedMemorySize, N::kGroups * N::kGroupBytes));
+  MLPSP_SHARED_MEMORY(N::kGroups * N::kGroupBytes, (const void*)k_mlp_tc<KEEP, BF16, H, TAB>);
   launch_chained(k_mlp_tc<KEEP, BF16, H, TAB>, dim3(grid), dim3(N::kThreads), N::kGroups * N::kGroupBytes, st, image, sc->freq, sc->att, dir_table,
                  reinterpret_cast<const float4*>(rec_in), work, counters, rec_out, rec_ext, out_mode, status);
   return MLPSP_OK;
@@ -979,9 +977,7 @@ template <bool BF16, int H>
 static int launch_mini(const char* image, const mlpsp_scene* sc, const RecIn* rec_in, const int4* work_small,
                        const int32_t* counters, float4* rec_out, int out_mode, int32_t* status, cudaStream_t st, int grid) {
   using M = MiniNet<H>;
-  static DeviceOnce attr_once;
-  if (attr_once.first())
-    MLPSP_CUDA_OK(cudaFuncSetAttribute(k_mlp_tc_mini<BF16, H>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::kSmemBytes));
+  MLPSP_SHARED_MEMORY(M::kSmemBytes, (const void*)k_mlp_tc_mini<BF16, H>);
   launch_chained(k_mlp_tc_mini<BF16, H>, dim3(grid), dim3(kMiniRows), M::kSmemBytes, st, image, sc->freq, sc->att, reinterpret_cast<const float4*>(rec_in),
                                                                 work_small, counters, rec_out, out_mode, status);
   return MLPSP_OK;

@@ -163,8 +163,9 @@ __device__ __forceinline__ void ns_end(const NsArgs& q) {
 constexpr int kNsWarpRows = 32, kNsPairRows = 64;
 constexpr int kNsWarpFew = 512, kNsPairFew = 256;
 constexpr int kNsWarpLong[2] = {1024, 800}, kNsPairLong = 384;       // warp: up to 16 rows, up to 32
-int launch_ns_warp(const NsArgs& q, cudaStream_t st);
-int launch_ns_pair(const NsArgs& q, cudaStream_t st);
-int launch_ns_cluster(const NsArgs& q, cudaStream_t st);
+// launch false: all that may fail before a launch, and no launch
+int launch_ns_warp(const NsArgs& q, cudaStream_t st, bool launch);
+int launch_ns_pair(const NsArgs& q, cudaStream_t st, bool launch);
+int launch_ns_cluster(const NsArgs& q, cudaStream_t st, bool launch);
 
 }  // namespace mlpsp

@@ -464,21 +464,21 @@ __global__ void __launch_bounds__(kNpThreads, CTAS) k_ns_pair(const NsArgs q, co
 }
 
 template <int NB, int CTAS>
-static int ns_pair(const NsArgs& q, cudaStream_t st) {
+static int ns_pair(const NsArgs& q, cudaStream_t st, bool launch) {
   constexpr int most = np_smem(NB ? (NB + 1) / 2 : kNsPairLong / 16);
   static_assert(most <= 227 * 1024 && (NB == 0 || CTAS * (most + 1024) <= 227 * 1024), "resident CTAs");
   const int smem = NB ? most : np_smem((q.large + 15) / 16);
-  static DeviceOnce once;
-  if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_pair<NB, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  MLPSP_SHARED_MEMORY(most, (const void*)k_ns_pair<NB, CTAS>);
   MLPSP_REQUIRE(q.count < (1ll << 31), MLPSP_E_LIMIT, "orthogonalize: too many matrices");
+  if (!launch) return MLPSP_OK;
   const bool prefetch = reinterpret_cast<uintptr_t>(q.w) % 16 == 0 && q.stride % 4 == 0;
   LaunchScope scope(kKMisc, 1, st);
   return cuda_check(launch_chained(k_ns_pair<NB, CTAS>, dim3((unsigned)q.count), dim3(kNpThreads), smem, st, q, prefetch), "orthogonalize");
 }
 
-int launch_ns_pair(const NsArgs& q, cudaStream_t st) {
+int launch_ns_pair(const NsArgs& q, cudaStream_t st, bool launch) {
   const int nb = (q.large + 7) / 8;
-  return nb <= 6 ? ns_pair<6, 6>(q, st) : nb <= 8 ? ns_pair<8, 6>(q, st) : nb <= 9 ? ns_pair<9, 6>(q, st) : nb <= 12 ? ns_pair<12, 5>(q, st) : ns_pair<0, 6>(q, st);
+  return (nb <= 6 ? ns_pair<6, 6> : nb <= 8 ? ns_pair<8, 6> : nb <= 9 ? ns_pair<9, 6> : nb <= 12 ? ns_pair<12, 5> : ns_pair<0, 6>)(q, st, launch);
 }
 
 }  // namespace mlpsp

@@ -453,15 +453,15 @@ static bool ns_many(const NsArgs& q) {
   return (q.count + pack - 1) / pack * ((q.large + kNtMaxCols - 1) / kNtMaxCols) > sm_count();
 }
 
-int launch_ns_cluster(const NsArgs& q, cudaStream_t st) {
+int launch_ns_cluster(const NsArgs& q, cudaStream_t st, bool launch) {
   const int cluster = nt_cluster(q);
   const int np = ((q.large + cluster - 1) / cluster + 15) / 16 * 16;
   const int pack = kNtRows / q.small;
   const int64_t tiles = (q.count + pack - 1) / pack;
   const int smem = nt_smem(np);
-  static DeviceOnce once;
-  if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, nt_smem(kNtMaxCols)));
+  MLPSP_SHARED_MEMORY(nt_smem(kNtMaxCols), (const void*)k_ns_cluster);
   MLPSP_REQUIRE(tiles * cluster < (1ll << 31), MLPSP_E_LIMIT, "orthogonalize: too many matrices");
+  if (!launch) return MLPSP_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * cluster));
   cfg.blockDim = dim3(kNtThreads);
@@ -500,9 +500,10 @@ static bool ns_bounded(double a, double b, double c, int steps) {
   return true;
 }
 
-// what the two entries share
+// what the two entries share; stage: how far to go
+enum NsStage { kNsCheck, kNsPrepare, kNsLaunch };
 static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a, double b, double c,
-                     double eps, cudaStream_t st, bool launch = true) {
+                     double eps, cudaStream_t st, NsStage stage) {
   MLPSP_REQUIRE(n >= 0 && rows >= 1 && cols >= 1, MLPSP_E_ARG, "%s: bad sizes", who);
   MLPSP_REQUIRE(std::min(rows, cols) <= MLPSP_MUON_MAX_SMALL && std::max(rows, cols) <= MLPSP_MUON_MAX_LARGE, MLPSP_E_LIMIT,
                 "%s: %d x %d matrices; at most %d on the smaller and %d on the larger side", who, rows, cols, MLPSP_MUON_MAX_SMALL,
@@ -514,7 +515,7 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
   MLPSP_REQUIRE(ns_bounded(a, b, c, steps), MLPSP_E_ARG, "%s: singular values leave [0, 4] with these coefficients", who);
   if (n == 0) return MLPSP_OK;
   MLPSP_REQUIRE(q.g && (q.m ? q.w != nullptr : q.out != nullptr), MLPSP_E_ARG, "%s: null pointer", who);
-  if (!launch) return MLPSP_OK;
+  if (stage == kNsCheck) return MLPSP_OK;
   const bool tall = rows > cols;
   q.count = n;
   q.stride = (int64_t)rows * cols;
@@ -535,11 +536,11 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
     for (int v = 2; v <= 4; v *= 2)
       if (cols % v == 0 && wide % (4 * v) == 0 && typed % (size * v) == 0) q.vec = v;
   if (q.small <= kNsWarpRows) {
-    if (q.large <= kNsWarpFew || (q.large <= kNsWarpLong[q.small > 16] && ns_many(q))) return launch_ns_warp(q, st);
+    if (q.large <= kNsWarpFew || (q.large <= kNsWarpLong[q.small > 16] && ns_many(q))) return launch_ns_warp(q, st, stage == kNsLaunch);
   } else if (q.small <= kNsPairRows) {
-    if (q.large <= kNsPairFew || (q.large <= kNsPairLong && ns_many(q))) return launch_ns_pair(q, st);
+    if (q.large <= kNsPairFew || (q.large <= kNsPairLong && ns_many(q))) return launch_ns_pair(q, st, stage == kNsLaunch);
   }
-  return launch_ns_cluster(q, st);
+  return launch_ns_cluster(q, st, stage == kNsLaunch);
 }
 
 }  // namespace mlpsp
@@ -583,9 +584,9 @@ extern "C" int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n,
   q.out = out;
   q.type = dtype;
   NsAnswer answer(gave_up_host);
-  int rc = ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream, false);
+  int rc = ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream, kNsCheck);
   if (!rc) rc = answer.open(q);
-  if (!rc) rc = ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream);
+  if (!rc) rc = ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream, kNsLaunch);
   return rc ? rc : answer.read((cudaStream_t)stream);
 }
 
@@ -597,10 +598,11 @@ extern "C" int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, 
   MLPSP_REQUIRE(lr >= 0.0 && lr < 1e30 && weight_decay >= 0.0 && weight_decay < 1e30, MLPSP_E_ARG,
                 "mlpsp_muon_step: lr and weight_decay must be finite and not negative");
   NsAnswer answer(gave_up_host);
-  for (int pass = 0; pass < 2; ++pass) {       // all tensors are checked before the first launch
+  // all tensors are checked, and their kernels allowed the shared memory that they take, before the first launch
+  for (const NsStage stage : {kNsCheck, kNsPrepare, kNsLaunch}) {
     bool follows = false;
     NsArgs shared = {};
-    if (pass == 1) {
+    if (stage == kNsLaunch) {
       const int rc = answer.open(shared);
       if (rc) return rc;
     }
@@ -620,7 +622,7 @@ extern "C" int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, 
       q.keep = (float)(1.0 - lr * weight_decay);
       q.step = (float)(lr * t.scale);
       q.follows = follows;
-      const int rc = ns_launch("mlpsp_muon_step", q, t.n, t.rows, t.cols, steps, a, b, c, eps, (cudaStream_t)stream, pass == 1);
+      const int rc = ns_launch("mlpsp_muon_step", q, t.n, t.rows, t.cols, steps, a, b, c, eps, (cudaStream_t)stream, stage);
       if (rc) return rc;
       follows |= t.n > 0;
     }

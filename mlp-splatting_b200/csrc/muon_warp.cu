@@ -551,25 +551,25 @@ __global__ void __launch_bounds__(32, CTAS) k_ns_warp(const NsArgs q, const int 
 }
 
 template <int MB, int NB, int CTAS>
-static int ns_warp(const NsArgs& q, cudaStream_t st) {
+static int ns_warp(const NsArgs& q, cudaStream_t st, bool launch) {
   constexpr int most = (NB ? (NB + 1) / 2 : kNsWarpLong[MB - 1] / 16) * ns_panel_bytes<MB>();
   static_assert(NB == 0 || CTAS * (most + 1024) <= 227 * 1024, "resident CTAs");
   const int smem = NB ? most : (q.large + 15) / 16 * ns_panel_bytes<MB>();
-  static DeviceOnce once;
-  if (once.first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(k_ns_warp<MB, NB, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  MLPSP_SHARED_MEMORY(most, (const void*)k_ns_warp<MB, NB, CTAS>);
   const int pack = std::max(1, 16 * MB / q.small);
   const int64_t tiles = (q.count + pack - 1) / pack;
   MLPSP_REQUIRE(tiles < (1ll << 31), MLPSP_E_LIMIT, "orthogonalize: too many matrices");
+  if (!launch) return MLPSP_OK;
   const bool prefetch = reinterpret_cast<uintptr_t>(q.w) % 16 == 0 && pack * q.stride % 4 == 0;
   LaunchScope scope(kKMisc, 1, st);
   return cuda_check(launch_chained(k_ns_warp<MB, NB, CTAS>, dim3((unsigned)tiles), dim3(32), smem, st, q, pack, prefetch), "orthogonalize");
 }
 
-int launch_ns_warp(const NsArgs& q, cudaStream_t st) {
+int launch_ns_warp(const NsArgs& q, cudaStream_t st, bool launch) {
   const int nb = (q.large + 7) / 8;
-  if (nb > 12) return q.small <= 16 ? ns_warp<1, 0, 24>(q, st) : ns_warp<2, 0, 16>(q, st);
-  if (q.small <= 16) return nb <= 4 ? ns_warp<1, 4, 32>(q, st) : nb <= 6 ? ns_warp<1, 6, 28>(q, st) : nb <= 9 ? ns_warp<1, 9, 28>(q, st) : ns_warp<1, 12, 28>(q, st);
-  return nb <= 4 ? ns_warp<2, 4, 16>(q, st) : nb <= 6 ? ns_warp<2, 6, 16>(q, st) : nb <= 9 ? ns_warp<2, 9, 16>(q, st) : ns_warp<2, 12, 16>(q, st);
+  auto* run = q.small <= 16 ? (nb <= 4 ? ns_warp<1, 4, 32> : nb <= 6 ? ns_warp<1, 6, 28> : nb <= 9 ? ns_warp<1, 9, 28> : nb <= 12 ? ns_warp<1, 12, 28> : ns_warp<1, 0, 24>)
+                            : (nb <= 4 ? ns_warp<2, 4, 16> : nb <= 6 ? ns_warp<2, 6, 16> : nb <= 9 ? ns_warp<2, 9, 16> : nb <= 12 ? ns_warp<2, 12, 16> : ns_warp<2, 0, 16>);
+  return run(q, st, launch);
 }
 
 }  // namespace mlpsp

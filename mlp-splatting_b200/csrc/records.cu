@@ -1564,13 +1564,9 @@ int launch_render_sorted(const mlpsp_scene* sc, const mlpsp_frame* fr, const Scr
     const int rc_ft = launch_feature_tc(sc, fr, s, used32, st);
     if (rc_ft) return rc_ft;
   } else if (want_feat) {
-    static DeviceOnce attr_once;
     const int CB = std::min(sc->feat_dim, kFeatChan);
     const size_t smem = sizeof(float) * 64 * (size_t)CB;
-    if (attr_once.first()) {
-      MLPSP_CUDA_OK(cudaFuncSetAttribute(k_feature_composite<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * kFeatChan * 4));
-      MLPSP_CUDA_OK(cudaFuncSetAttribute(k_feature_composite<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * kFeatChan * 4));
-    }
+    MLPSP_SHARED_MEMORY(64 * kFeatChan * 4, (const void*)k_feature_composite<false>, (const void*)k_feature_composite<true>);
     LaunchScope scope(kKComposite, 1, st);
     const dim3 grid(T, (sc->feat_dim + CB - 1) / CB);
     const bool vec = sc->feat_dim >= kFeatChan && (sc->feat_dim & 3) == 0 && (reinterpret_cast<uintptr_t>(sc->feat_attr) & 15) == 0;

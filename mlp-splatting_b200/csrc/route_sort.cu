@@ -17,7 +17,7 @@
 namespace mlpsp {
 
 constexpr int kRsBits = 9, kRsBins = 1 << kRsBits, kRsThreads = kRsBins, kRsWarps = kRsThreads / 32;
-constexpr int kRsRounds = 8, kRsItems = kRsThreads * kRsRounds;
+constexpr int kRsRounds = 8, kRsItems = kRsThreads * kRsRounds, kRsItemBytes = kRsItems * (int)sizeof(uint2);
 
 // an id outside [0, nprim) sorts behind every primitive, as key nprim
 template <bool FIRST>
@@ -312,6 +312,7 @@ extern "C" int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_rec
   const RsLayout L = rs_layout(R, n);
   MLPSP_REQUIRE(L.bytes == 0 || (scratch && scratch_bytes >= L.bytes), MLPSP_E_SCRATCH, "%s: scratch needs %lld bytes", who, (long long)L.bytes);
   cudaStream_t st = (cudaStream_t)stream;
+  MLPSP_SHARED_MEMORY(kRsItemBytes, (const void*)k_rs_place<true, false>, (const void*)k_rs_place<false, false>);
   HostWords& hw = host_words();
   cudaEvent_t ev = nullptr;
   if (findings_host) {
@@ -349,11 +350,7 @@ extern "C" int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_rec
       launch_chained(first ? k_rs_count<true> : k_rs_count<false>, dim3(p.nblocks), dim3(kRsThreads), 0, st, k_in, R, n, shift, mask, p.nblocks, counts);
       launch_chained(k_rs_scan, dim3(mask + 1), dim3(kRsThreads), 0, st, p.nblocks, counts, totals);
       auto* place = first ? (last ? k_rs_place<true, true> : k_rs_place<true, false>) : (last ? k_rs_place<false, true> : k_rs_place<false, false>);
-      const int smem = last ? 0 : (int)sizeof(uint2) * kRsItems;
-      if (!last) {
-        static DeviceOnce once[2];
-        if (once[first].first()) MLPSP_CUDA_OK(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-      }
+      const int smem = last ? 0 : kRsItemBytes;
       launch_chained(place, dim3(p.nblocks), dim3(kRsThreads), smem, st, k_in, v_in, R, n, shift, mask, p.nblocks, counts, totals, k_out, v_out, slots,
                      p.passes == 1 ? offsets : nullptr, starts);
       k_in = k_out;

@@ -532,13 +532,8 @@ __global__ void __launch_bounds__(kVjpRows, kVjpCtas) k_grouped_vjp_tc(
 int launch_grouped_vjp_tc(bool bf16, const float* x6, const float* d4, const int32_t* masks, const VjpItem* items,
                           int64_t max_items, const VjpItem* multi, int32_t* counters, const mlpsp_scene* sc, float scale,
                           const VjpOut& out, float* partial, cudaStream_t st) {
-  static DeviceOnce attr_once;
-  if (attr_once.first()) {
-    MLPSP_CUDA_OK(cudaFuncSetAttribute(k_grouped_vjp_tc<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVjpSmem));
-    MLPSP_CUDA_OK(cudaFuncSetAttribute(k_grouped_vjp_tc<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVjpSmem));
-    MLPSP_CUDA_OK(cudaFuncSetAttribute(k_grouped_vjp_tc<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVjpSmem));
-    MLPSP_CUDA_OK(cudaFuncSetAttribute(k_grouped_vjp_tc<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kVjpSmem));
-  }
+  MLPSP_SHARED_MEMORY(kVjpSmem, (const void*)k_grouped_vjp_tc<false, false>, (const void*)k_grouped_vjp_tc<false, true>,
+                      (const void*)k_grouped_vjp_tc<true, false>, (const void*)k_grouped_vjp_tc<true, true>);
   auto* kernel = bf16 ? (masks ? k_grouped_vjp_tc<true, true> : k_grouped_vjp_tc<true, false>)
                       : (masks ? k_grouped_vjp_tc<false, true> : k_grouped_vjp_tc<false, false>);
   const int vec = ((reinterpret_cast<uintptr_t>(sc->W1) | reinterpret_cast<uintptr_t>(sc->W2)) & 15) == 0 &&

@@ -452,7 +452,8 @@ int mlpsp_weight_gradients(const mlpsp_scene* scene, const int64_t* offsets, con
  * NaN, alone.  Coefficients under which singular values leave [0, 4] within the steps are refused, as are more than
  * MLPSP_MUON_MAX_SMALL rows or columns on the shorter and MLPSP_MUON_MAX_LARGE on the longer side; 1e-15 <= eps <= 1, 1 <= steps <= 32.
  * gave_up_host (HOST, or NULL) receives 1 when a device-side wait gave up, results then invalid, else 0, for which the call waits; only
- * shapes for which mlpsp_orthogonalize_waits answers 1 wait. */
+ * shapes for which mlpsp_orthogonalize_waits answers 1 wait.  What such a wait leaves without a result is NaN, with or without
+ * gave_up_host. */
 #define MLPSP_MUON_MAX_SMALL 128
 #define MLPSP_MUON_MAX_LARGE 2048
 int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols);
@@ -461,7 +462,8 @@ int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n, int32_t ro
 /* One step, in place, on the weight matrices of `count` tensors and their momenta (FP32): m <- m + (1 - momentum)(g - m),
  * U = g + momentum (m - g) (nesterov) or m, w <- (1 - lr weight_decay) w - lr scale X(U), X as above.
  * active [n] (bytes, or NULL; then every tensor's n is the same): matrices whose byte is zero keep weights and momenta and are not
- * read.  No weights or momenta may overlap any other array of the call: the tensors' launches run side by side. */
+ * read.  No weights or momenta may overlap any other array of the call: the tensors' launches run side by side.  Where a device-side
+ * wait gave up the weights become NaN; momenta are updated before the iteration, whose waits these are. */
 typedef struct mlpsp_muon_tensor {
   float* weights;            /* [n, rows, cols] */
   const void* grads;         /* the same, of grad_dtype (MLPSP_PRECISION_*) */
@@ -473,6 +475,10 @@ typedef struct mlpsp_muon_tensor {
 } mlpsp_muon_tensor;
 int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, const uint8_t* active, double lr, double momentum, int32_t nesterov,
                     double weight_decay, int32_t steps, double a, double b, double c, double eps, int32_t* gave_up_host, void* stream);
+
+/* For tests of a caller's failure handling: in the following calls of this host thread the first thread block of every kernel with bounded waits
+ * leaves its product number `product` (1, 2, ... three a step) unanswered, so that the wait for it gives up after a second.  0: none. */
+int mlpsp_test_withhold_answer(int32_t product);
 
 /* ---- the step after the feature map: feature decoder and text query ---- */
 

@@ -96,6 +96,7 @@ _SIGS = {
     "mlpsp_orthogonalize": (C.c_int, [_fp, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32] + [C.c_double] * 4 + [_fp, _fp, _fp]),
     "mlpsp_muon_step": (C.c_int, [C.POINTER(MuonTensor), C.c_int32, _fp, C.c_double, C.c_double, C.c_int32, C.c_double, C.c_int32]
                         + [C.c_double] * 4 + [_fp, _fp]),
+    "mlpsp_test_withhold_answer": (C.c_int, [C.c_int32]),
     "mlpsp_decoder_packed_bytes": (C.c_int64, [C.POINTER(Decoder), C.c_int32]),
     "mlpsp_pack_decoder": (C.c_int, [C.POINTER(Decoder), C.c_int32, _fp, _fp, _fp]),
     "mlpsp_decode_features": (C.c_int, [C.POINTER(Decoder), C.c_int32, _fp, _fp, C.c_int32, C.c_int32, _fp, _fp, _fp, _fp]),

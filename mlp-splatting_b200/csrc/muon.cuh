@@ -24,6 +24,7 @@ struct NsArgs {
   void* out;                 // result, in g's type
   const uint8_t* active;     // [count], or null
   volatile int32_t* gave_up; // page-locked host word that a wait which gives up sets (the cluster kernel), or null
+  int32_t withhold;          // this product of the first CTA is not answered (mlpsp_test_withhold_answer), or 0
   int64_t count, stride;     // matrices, elements of each
   int32_t type;              // element type of g and out (MLPSP_PRECISION_*)
   int32_t small, large;      // X is small x large

@@ -6,7 +6,8 @@
 // computed by each.  Matrices of few rows are stacked (four of 32): the blocks of A off their diagonal are cleared, after which
 // everything stays block-diagonal.  Accumulators (A | A^2, later the new slice in the same columns) are in tensor memory.
 //
-// Every wait on an mbarrier is bounded; one that gives up is reported to the host, and this CTA's slice of the result is not written.
+// Every wait on an mbarrier is bounded.  A CTA in which one gives up issues no further products, hands NaN to its cluster, makes its slice of
+// the result NaN, waits once more (bounded too) for the products it had issued before it frees their tensor memory, and tells the host.
 #include <cmath>
 #include "muon.cuh"
 
@@ -96,24 +97,32 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
   const int groups = np / 16;                                      // of 16 columns; a thread has part, part + 4, ...
   const int col0 = (int)rank * np;
   uint32_t phase = 0u;
-  bool ok = true;
+  bool ok = true, late = false;      // ok: the same in all threads behind ready(); late: this warp's last wait gave up
+  int products = 0;
 
   auto wait = [&] {
-    if (ok && !mbar_wait(bar, phase)) ok = false;      // after one that gave up the others are not waited for
-    phase ^= 1u;
+    if (ok) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar, phase));
+      late = !ok;
+      if (late) s_word[3] = 1u;
+      if (ok) phase ^= 1u;
+    }
     tc_fence_after();
   };
-  // everyone's operand writes are in place: make them visible to the tensor cores and let one thread go on
+  // everyone's operand writes are in place: make them visible to the tensor cores and let one thread go on; tells the CTA of a wait that
+  // gave up
   auto ready = [&] {
     fence_async_smem();
     tc_fence_before();
     __syncthreads();
+    ok = ok && *const_cast<volatile uint32_t*>(s_word + 3) == 0u;
     tc_fence_after();
   };
   // `steps` pairs of operands that lie `da` and `db` bytes apart: lo hi and hi lo products, then hi hi (the tensor core rounds a sum towards
   // zero with every MMA, so the small ones come first)
   auto product = [&](uint32_t to, uint64_t a_hi, uint64_t a_lo, uint64_t b_hi, uint64_t b_lo, int steps, int da, int db, uint32_t idesc) {
-    if (warp == 0) {
+    ++products;
+    if (warp == 0 && ok) {
       if (elect_one()) {
         for (int s = 0; s < steps; ++s) {
           const uint64_t oa = (uint64_t)(s * da >> 4), ob = (uint64_t)(s * db >> 4);
@@ -121,7 +130,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
           mma_f16(to, a_lo + oa, b_hi + ob, idesc, 1u);
         }
         for (int s = 0; s < steps; ++s) mma_f16(to, a_hi + (uint64_t)(s * da >> 4), b_hi + (uint64_t)(s * db >> 4), idesc, 1u);
-        mma_commit(bar);
+        if (products != q.withhold || blockIdx.x != 0) mma_commit(bar);
       }
       __syncwarp();
     }
@@ -281,6 +290,9 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (gr * 16 + e == row) d[e] = __float_as_uint(xx);
+          if (!ok)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) d[e] = 0x7fffffffu;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             *reinterpret_cast<uint4*>(pah + (gr * 4 + e) * kNtChunk) = make_uint4(d[4 * e], d[4 * e + 1], d[4 * e + 2], d[4 * e + 3]);
@@ -367,11 +379,8 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
       for (int w = 0; w < kNtParts; ++w) own = fmaf(by.c, s_asq[w * kNtRows + row], own);
       xsq = 0.f;
       wait();
-      if (last) {
-        if (!ok) atomicOr(s_word + 3, 1u);
-        __syncthreads();
-      }
-      const bool write = last && in && s_word[3] == 0u;
+      if (last) ok = __syncthreads_and(ok) != 0;
+      const bool write = last && in;
       for (int gr = part; gr < groups; gr += kNtParts) {
         char* const ph = pxh + gr * 2 * kNtChunk;
         char* const pl = pxl + gr * 2 * kNtChunk;
@@ -398,7 +407,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
           nt_put(ph, pl, h, l);
         }
         if (!write) continue;
-        const float fin = lost ? __int_as_float(0x7fffffff) : ns_exp2i(-10 - k2);
+        const float fin = lost || !ok ? __int_as_float(0x7fffffff) : ns_exp2i(-10 - k2);
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] *= fin;
         if (q.vec == 4) {
@@ -431,6 +440,7 @@ __global__ void __launch_bounds__(kNtThreads) k_ns_cluster(const NsArgs q, const
   };
   work();
   if (!ok && q.gave_up) *q.gave_up = 1;
+  if (late) mbar_wait(bar, phase);
   __syncthreads();
   if (warp == 0) tmem_free(tmem, kNtTmemCols);
   if (cluster > 1) nt_cluster_sync();      // no CTA leaves while another may read its shared memory
@@ -548,6 +558,8 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
 using namespace mlpsp;
 
 namespace mlpsp {
+static thread_local int32_t g_withhold = 0;
+
 // the answer of a call's waits, for which the call waits
 struct NsAnswer {
   int32_t* to;
@@ -572,6 +584,12 @@ struct NsAnswer {
 };
 }  // namespace mlpsp
 
+extern "C" int mlpsp_test_withhold_answer(int32_t product) {
+  MLPSP_REQUIRE(product >= 0, MLPSP_E_ARG, "mlpsp_test_withhold_answer: product must not be negative");
+  g_withhold = product;
+  return MLPSP_OK;
+}
+
 extern "C" int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols) {
   const int small = std::min(rows, cols), large = std::max(rows, cols);
   return small > kNsPairRows || large > (small <= kNsWarpRows ? kNsWarpFew : kNsPairFew) ? 1 : 0;
@@ -583,6 +601,7 @@ extern "C" int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n,
   q.g = update;
   q.out = out;
   q.type = dtype;
+  q.withhold = g_withhold;
   NsAnswer answer(gave_up_host);
   int rc = ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream, kNsCheck);
   if (!rc) rc = answer.open(q);
@@ -616,6 +635,7 @@ extern "C" int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, 
       q.w = t.weights;
       q.active = active;
       q.type = t.grad_dtype;
+      q.withhold = g_withhold;
       q.nesterov = nesterov != 0;
       q.momentum = (float)momentum;
       q.rest = (float)(1.0 - momentum);

@@ -77,8 +77,8 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     apart from it) receives the result in update's type.  The iteration has FP32 accuracy whatever the type.  A matrix of zeros stays
     zero; one that holds an infinity or a NaN becomes NaN and touches no other.  Coefficients under which singular values leave
     [0, 4] are refused.  Large matrices (more than 64 rows on the shorter side, or more than 512, with 33 to 64 rows 256, on the
-    longer) may go to a kernel with bounded waits, for whose answer the call waits unless check is False; their number decides on the
-    kernel and on the CTAs that share a matrix, which shows in the last bits."""
+    longer) may go to a kernel with bounded waits, for whose answer the call waits (RuntimeError if one gave up) unless check is False, where
+    only NaN in the result shows it; their number decides on the kernel and on the CTAs that share a matrix, which shows in the last bits."""
     n, rows, cols = _shape("update", update)
     if update.dtype not in _TYPES:
         raise ValueError("update must be float32, float16 or bfloat16")
@@ -112,7 +112,7 @@ def muon_step(weights, grads, momenta, *, lr: float, momentum: float = 0.95, nes
     csr.offsets[1:] == csr.offsets[:-1]) keep weights and momenta; their gradients are not read.  The orthogonalised update does not
     shrink with the gradient, so a primitive that is not left out moves by lr however little it was seen; a zero gradient and
     zero momentum leave its direction at zero.  A gradient that is not finite makes its own matrix NaN: check gradients first, as
-    grouped_weight_gradients does."""
+    grouped_weight_gradients does.  check: as in orthogonalize; without it a wait that gave up shows as NaN in the weights."""
     lists = [[t] if torch.is_tensor(t) else list(t) for t in (weights, grads, momenta)]
     if not lists[0] or len({len(k) for k in lists}) != 1:
         raise ValueError("weights, grads and momenta must be as many, at least one")

@@ -11,6 +11,7 @@ from dataclasses import dataclass
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -21,6 +22,13 @@ TILE_CAPACITY = 1536  # MLPSP_TILE_CANDIDATE_CAPACITY default of the reference l
 def _stream_ptr(device):
     """cudaStream_t of the current stream, without the torch.cuda.Stream object around it (two microseconds of every call)."""
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+
+
+def _refuse_tangents(what, tensors):
+    """For operators without a forward-mode derivative: dropped silently, a tangent would read as a derivative of zero.  (A dual tensor does not
+    require grad, and no_grad leaves forward mode on.)"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative; an input carries a tangent")
 
 
 class _on:

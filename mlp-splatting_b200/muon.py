@@ -14,7 +14,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib as L
-from .engine import _on, _stream_ptr
+from .engine import _on, _refuse_tangents, _stream_ptr
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)      # (a, b, c): five steps take singular values from 0.01 .. 1 to 0.7 .. 1.2
 _TYPES = {torch.float32: L.PRECISION_F32, torch.float16: L.PRECISION_F16, torch.bfloat16: L.PRECISION_BF16}
@@ -76,9 +76,10 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     update: float32, float16 or bfloat16, [rows, columns] or [N, rows, columns], contiguous; out (update itself, or a tensor
     apart from it) receives the result in update's type.  The iteration has FP32 accuracy whatever the type.  A matrix of zeros stays
     zero; one that holds an infinity or a NaN becomes NaN and touches no other.  Coefficients under which singular values leave
-    [0, 4] are refused.  Large matrices (more than 64 rows on the shorter side, or more than 512, with 33 to 64 rows 256, on the
+    [0, 4] are refused.  There is no gradient: the result does not require grad, and inputs with forward-mode tangents are refused.  Large matrices (more than 64 rows on the shorter side, or more than 512, with 33 to 64 rows 256, on the
     longer) may go to a kernel with bounded waits, for whose answer the call waits (RuntimeError if one gave up) unless check is False, where
     only NaN in the result shows it; their number decides on the kernel and on the CTAs that share a matrix, which shows in the last bits."""
+    _refuse_tangents("orthogonalize", (update, out))
     n, rows, cols = _shape("update", update)
     if update.dtype not in _TYPES:
         raise ValueError("update must be float32, float16 or bfloat16")
@@ -116,6 +117,7 @@ def muon_step(weights, grads, momenta, *, lr: float, momentum: float = 0.95, nes
     lists = [[t] if torch.is_tensor(t) else list(t) for t in (weights, grads, momenta)]
     if not lists[0] or len({len(k) for k in lists}) != 1:
         raise ValueError("weights, grads and momenta must be as many, at least one")
+    _refuse_tangents("muon_step", (t for k in lists for t in k))
     shapes = [_shape("weights", w) for w in lists[0]]
     for w, g, m in zip(*lists):
         if w.dtype != torch.float32 or m.dtype != torch.float32:

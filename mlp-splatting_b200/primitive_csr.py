@@ -11,7 +11,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib as L
-from .engine import _on, _stream_ptr
+from .engine import _on, _refuse_tangents, _stream_ptr
 
 
 @dataclass
@@ -289,7 +289,8 @@ class _CombineRows(torch.autograd.Function):
 def dispatch_rows(x: torch.Tensor, route: RecordRoute) -> torch.Tensor:
     """Every pixel's row to its records, grouped by primitive: out[route.slots[r]] = x[pixel of r]; the rows of dropped
     records, from route.offsets[N] on, are zero.  x [pixels, D] float32, float16 or bfloat16, contiguous; out [records, D].
-    Differentiable in x; dispatch_rows_gradient is the gradient without autograd."""
+    Differentiable in x (reverse mode, once); dispatch_rows_gradient is the gradient without autograd."""
+    _refuse_tangents("dispatch_rows", (x,))
     if torch.is_grad_enabled() and x.requires_grad:
         return _DispatchRows.apply(x, route)
     return _dispatch(x, route)
@@ -299,6 +300,7 @@ def dispatch_rows(x: torch.Tensor, route: RecordRoute) -> torch.Tensor:
 def dispatch_rows_gradient(grad_rows: torch.Tensor, route: RecordRoute) -> torch.Tensor:
     """Gradient of dispatch_rows with respect to x [pixels, D]: the sums of every pixel's records' rows of grad_rows [records, D],
     in FP32 in the order of the records, rounded once; rows of dropped records are not read."""
+    _refuse_tangents("dispatch_rows_gradient", (grad_rows,))
     return _combine(grad_rows, route, None, "grad_rows")
 
 
@@ -306,8 +308,9 @@ def combine_rows(y: torch.Tensor, route: RecordRoute, weights: torch.Tensor | No
     """The records' rows back to their pixels: out[p] = sum of weights[r] * y[route.slots[r]] over the records r of p (ones
     without weights), in FP32 in the order of the records, rounded once to y's type.  y [records, D] grouped by primitive,
     float32, float16 or bfloat16, contiguous; weights float32, one per record in record order ([pixels, fan] or [records]).  Rows
-    of dropped records are not read; a pixel without records gets zeros.  Differentiable in y and weights;
-    combine_rows_gradients gives both gradients without autograd."""
+    of dropped records are not read; a pixel without records gets zeros.  Differentiable in y and weights
+    (reverse mode, once); combine_rows_gradients gives both gradients without autograd."""
+    _refuse_tangents("combine_rows", (y, weights))
     if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
         return _CombineRows.apply(y, route, weights)
     return _combine(y, route, weights)
@@ -317,4 +320,5 @@ def combine_rows(y: torch.Tensor, route: RecordRoute, weights: torch.Tensor | No
 def combine_rows_gradients(grad_out: torch.Tensor, y: torch.Tensor, route: RecordRoute, weights: torch.Tensor | None = None):
     """(gradient of combine_rows with respect to y [records, D], with respect to weights in their shape, or None without
     weights) from grad_out [pixels, D].  Zero for dropped records."""
+    _refuse_tangents("combine_rows_gradients", (grad_out, y, weights))
     return _combine_gradients(grad_out, y, route, weights, True, weights is not None)

@@ -491,14 +491,13 @@ int launch_ns_cluster(const NsArgs& q, cudaStream_t st, bool launch) {
 
 // Whether the iteration stays in the binary16 range of the scaled operands: from singular values in [0, 1], values within [-4, 4] and
 // |b s^2 + c s^4| within 32 after every step.  Both polynomials take their extremes over [0, top] at the ends or where their
-// derivatives vanish, quadratics in s^2.
+// derivatives vanish, quadratics in s^2: that of a s + b s^3 + c s^5 has the roots q / (5 c) and a / q, neither a difference of near numbers.
 static bool ns_bounded(double a, double b, double c, int steps) {
   double top = 1.0;
   for (int it = 0; it < steps; ++it) {
     double next = 0.0;
-    const double disc = 9.0 * b * b - 20.0 * a * c, root = disc > 0.0 ? std::sqrt(disc) : 0.0;
-    const double at[] = {top * top, c != 0.0 ? -b / (2.0 * c) : 0.0, c != 0.0 ? (-3.0 * b + root) / (10.0 * c) : b != 0.0 ? -a / (3.0 * b) : 0.0,
-                         c != 0.0 ? (-3.0 * b - root) / (10.0 * c) : 0.0};
+    const double disc = 9.0 * b * b - 20.0 * a * c, q = -0.5 * (3.0 * b + std::copysign(disc > 0.0 ? std::sqrt(disc) : 0.0, b));
+    const double at[] = {top * top, c != 0.0 ? -b / (2.0 * c) : 0.0, c != 0.0 ? q / (5.0 * c) : 0.0, q != 0.0 ? a / q : 0.0};
     for (double s2 : at) {
       s2 = s2 > 0.0 && s2 < top * top ? s2 : top * top;
       const double p = b * s2 + c * s2 * s2, y = (a + p) * std::sqrt(s2);

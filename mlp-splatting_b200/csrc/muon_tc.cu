@@ -627,6 +627,7 @@ extern "C" int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, 
     for (int32_t i = 0; i < count; ++i) {
       const mlpsp_muon_tensor& t = tensors[i];
       MLPSP_REQUIRE(t.n <= 0 || (t.weights && t.grads && t.momenta), MLPSP_E_ARG, "mlpsp_muon_step: null pointer");
+      MLPSP_REQUIRE(!active || t.n == tensors[0].n, MLPSP_E_ARG, "mlpsp_muon_step: with active, all tensors must have as many matrices");
       MLPSP_REQUIRE(t.scale > 0.0 && t.scale < 1e30, MLPSP_E_ARG, "mlpsp_muon_step: scale must be finite and positive");
       NsArgs q = shared;
       q.g = t.grads;

@@ -342,7 +342,7 @@ int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_records, int32
 /* In the three calls below the records of pixel p are fan * p .. fan * (p + 1) - 1 (pixel_offsets NULL, records = pixels * fan)
  * or pixel_offsets[p] .. pixel_offsets[p + 1] - 1 (int64 [pixels + 1], from zero to records, ascending); slots and kept =
  * offsets + n (DEVICE pointer) are those of mlpsp_route_records.  dtype: MLPSP_PRECISION_F32 / _F16 / _BF16, the element type of
- * the rows; dim <= MLPSP_ROUTE_MAX_DIM.  Sums are taken in FP32 in the order of a pixel's records and rounded once; no atomics.
+ * the rows; dim <= MLPSP_ROUTE_MAX_DIM; pointers aligned to their elements.  Sums are taken in FP32 in the order of a pixel's records and rounded once; no atomics.
  * Offsets or slots that break these rules are never followed out of the arrays; the rows they reach are undefined. */
 #define MLPSP_ROUTE_MAX_DIM 65536
 /* out[slots[r], :] = x[pixel(r), :]; the rows of dropped records are zero.  x [pixels, dim], out [records, dim]. */

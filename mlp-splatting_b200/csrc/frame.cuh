@@ -196,6 +196,13 @@ int cuda_check(cudaError_t e, const char* what);
     if (!(cond)) { ::mlpsp::set_error(__VA_ARGS__); return (code); }\
   } while (0)
 
+// whether every pointer (a null one too) is a multiple of `bytes`
+inline bool aligned_to(int64_t bytes, std::initializer_list<const void*> ptrs) {
+  uintptr_t all = 0;
+  for (const void* p : ptrs) all |= reinterpret_cast<uintptr_t>(p);
+  return all % (uintptr_t)bytes == 0;
+}
+
 // SMs of the current device (asked once per device)
 int sm_count();
 

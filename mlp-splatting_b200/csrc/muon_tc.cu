@@ -524,6 +524,8 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
   MLPSP_REQUIRE(ns_bounded(a, b, c, steps), MLPSP_E_ARG, "%s: singular values leave [0, 4] with these coefficients", who);
   if (n == 0) return MLPSP_OK;
   MLPSP_REQUIRE(q.g && (q.m ? q.w != nullptr : q.out != nullptr), MLPSP_E_ARG, "%s: null pointer", who);
+  MLPSP_REQUIRE(aligned_to(q.type == MLPSP_PRECISION_F32 ? 4 : 2, {q.g, q.out}) && aligned_to(4, {q.m, q.w}), MLPSP_E_ARG,
+                "%s: a pointer is not aligned to its elements", who);
   if (stage == kNsCheck) return MLPSP_OK;
   const bool tall = rows > cols;
   q.count = n;

@@ -255,7 +255,8 @@ static int rt_piece(int64_t row_bytes, std::initializer_list<const void*> ptrs) 
   return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 
-static int rt_check(const char* who, const RouteView& v, int64_t dim, int32_t dtype) {
+static int rt_check(const char* who, const RouteView& v, int64_t dim, int32_t dtype, std::initializer_list<const void*> rows,
+                    std::initializer_list<const void*> floats) {
   MLPSP_REQUIRE(dtype == MLPSP_PRECISION_F32 || dtype == MLPSP_PRECISION_F16 || dtype == MLPSP_PRECISION_BF16, MLPSP_E_ARG,
                 "%s: unknown element type %d", who, dtype);
   MLPSP_REQUIRE(v.pixels >= 0 && v.records >= 0 && v.fan >= 0 && dim >= 1, MLPSP_E_ARG, "%s: bad sizes", who);
@@ -263,6 +264,8 @@ static int rt_check(const char* who, const RouteView& v, int64_t dim, int32_t dt
                 "%s: more than 2^31-1 pixels or records, or rows longer than %d", who, MLPSP_ROUTE_MAX_DIM);
   MLPSP_REQUIRE(v.pixel_offsets || v.pixels * v.fan == v.records, MLPSP_E_ARG, "%s: the record count is not pixels x fan", who);
   MLPSP_REQUIRE(v.kept && (v.records == 0 || v.slots), MLPSP_E_ARG, "%s: null pointer", who);
+  MLPSP_REQUIRE(aligned_to(dtype == MLPSP_PRECISION_F32 ? 4 : 2, rows) && aligned_to(4, floats) && aligned_to(4, {v.slots}) &&
+                aligned_to(8, {v.pixel_offsets, v.kept}), MLPSP_E_ARG, "%s: a pointer is not aligned to its elements", who);
   return MLPSP_OK;
 }
 
@@ -343,7 +346,7 @@ using namespace mlpsp;
 extern "C" int mlpsp_dispatch_rows(const void* x, int32_t dtype, int64_t dim, int64_t pixels, int32_t fan, const int64_t* pixel_offsets,
                                    const int32_t* slots, int64_t records, const int64_t* kept, void* out, void* stream) {
   const RouteView v{pixel_offsets, slots, kept, pixels, records, fan};
-  const int rc = rt_check("mlpsp_dispatch_rows", v, dim, dtype);
+  const int rc = rt_check("mlpsp_dispatch_rows", v, dim, dtype, {x, out}, {});
   if (rc) return rc;
   if (pixels == 0 || records == 0) return MLPSP_OK;
   MLPSP_REQUIRE(x && out, MLPSP_E_ARG, "mlpsp_dispatch_rows: null pointer");
@@ -363,7 +366,7 @@ extern "C" int mlpsp_combine_rows(const void* y, int32_t dtype, int64_t dim, con
                                   const int64_t* pixel_offsets, const int32_t* slots, int64_t records, const int64_t* kept, void* out,
                                   void* stream) {
   const RouteView v{pixel_offsets, slots, kept, pixels, records, fan};
-  const int rc = rt_check("mlpsp_combine_rows", v, dim, dtype);
+  const int rc = rt_check("mlpsp_combine_rows", v, dim, dtype, {y, out}, {weights});
   if (rc) return rc;
   if (pixels == 0) return MLPSP_OK;
   MLPSP_REQUIRE(out && (y || records == 0), MLPSP_E_ARG, "mlpsp_combine_rows: null pointer");
@@ -381,7 +384,7 @@ extern "C" int mlpsp_combine_rows_gradients(const void* grad_out, const void* y,
                                             int64_t pixels, int32_t fan, const int64_t* pixel_offsets, const int32_t* slots,
                                             int64_t records, const int64_t* kept, void* grad_y, float* grad_weights, void* stream) {
   const RouteView v{pixel_offsets, slots, kept, pixels, records, fan};
-  const int rc = rt_check("mlpsp_combine_rows_gradients", v, dim, dtype);
+  const int rc = rt_check("mlpsp_combine_rows_gradients", v, dim, dtype, {grad_out, y, grad_y}, {weights, grad_weights});
   if (rc) return rc;
   if (pixels == 0 || records == 0) return MLPSP_OK;
   MLPSP_REQUIRE(grad_out && (grad_y || grad_weights) && (y || !grad_weights), MLPSP_E_ARG, "mlpsp_combine_rows_gradients: null pointer");

@@ -309,6 +309,8 @@ extern "C" int mlpsp_route_records(const int32_t* primitive_ids, int64_t num_rec
   MLPSP_REQUIRE(R < (1ll << 31) && n < 2147483647, MLPSP_E_LIMIT, "%s: more than 2^31-1 records or primitives", who);
   MLPSP_REQUIRE(R == 0 || (primitive_ids && slots), MLPSP_E_ARG, "%s: null pointer", who);
   MLPSP_REQUIRE(!findings_host || (pixel_offsets && pixels >= 0), MLPSP_E_ARG, "%s: no pixel offsets to check", who);
+  MLPSP_REQUIRE(aligned_to(4, {primitive_ids, slots, scratch}) && aligned_to(8, {offsets, pixel_offsets}), MLPSP_E_ARG,
+                "%s: a pointer is not aligned to its elements", who);
   const RsLayout L = rs_layout(R, n);
   MLPSP_REQUIRE(L.bytes == 0 || (scratch && scratch_bytes >= L.bytes), MLPSP_E_SCRATCH, "%s: scratch needs %lld bytes", who, (long long)L.bytes);
   cudaStream_t st = (cudaStream_t)stream;

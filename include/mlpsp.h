@@ -451,12 +451,14 @@ int mlpsp_weight_gradients(const mlpsp_scene* scene, const int64_t* offsets, con
  * accuracy whatever the type, and the result is rounded once.  A matrix of zeros gives zeros, one that holds an infinity or a NaN gives
  * NaN, alone.  Coefficients under which singular values leave [0, 4] within the steps are refused, as are more than
  * MLPSP_MUON_MAX_SMALL rows or columns on the shorter and MLPSP_MUON_MAX_LARGE on the longer side; 1e-15 <= eps <= 1, 1 <= steps <= 32.
- * gave_up_host (HOST, or NULL) receives 1 when a device-side wait gave up, results then invalid, else 0, for which the call waits; only
- * shapes for which mlpsp_orthogonalize_waits answers 1 wait.  What such a wait leaves without a result is NaN, with or without
+ * gave_up_host (HOST, or NULL) receives 1 when a device-side wait gave up, results then invalid, for which the call waits, else 0; only n
+ * matrices for which mlpsp_orthogonalize_stack_waits answers 1 wait (on the current device; shapes for which mlpsp_orthogonalize_waits answers 0
+ * never do).  What such a wait leaves without a result is NaN, with or without
  * gave_up_host. */
 #define MLPSP_MUON_MAX_SMALL 128
 #define MLPSP_MUON_MAX_LARGE 2048
 int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols);
+int mlpsp_orthogonalize_stack_waits(int64_t n, int32_t rows, int32_t cols);
 int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a, double b,
                         double c, double eps, void* out, int32_t* gave_up_host, void* stream);
 /* One step, in place, on the weight matrices of `count` tensors and their momenta (FP32): m <- m + (1 - momentum)(g - m),

@@ -93,6 +93,7 @@ _SIGS = {
     "mlpsp_weight_gradients": (C.c_int, [C.POINTER(Scene), _fp, _fp, _fp, _fp, C.c_int64, C.c_int32, C.c_int32, C.c_float,
                                          _fp, _fp, _fp, _fp, _fp, _fp, _fp, C.c_int64, _fp, _fp]),
     "mlpsp_orthogonalize_waits": (C.c_int, [C.c_int32, C.c_int32]),
+    "mlpsp_orthogonalize_stack_waits": (C.c_int, [C.c_int64, C.c_int32, C.c_int32]),
     "mlpsp_orthogonalize": (C.c_int, [_fp, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32] + [C.c_double] * 4 + [_fp, _fp, _fp]),
     "mlpsp_muon_step": (C.c_int, [C.POINTER(MuonTensor), C.c_int32, _fp, C.c_double, C.c_double, C.c_int32, C.c_double, C.c_int32]
                         + [C.c_double] * 4 + [_fp, _fp]),

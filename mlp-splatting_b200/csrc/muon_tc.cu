@@ -457,10 +457,19 @@ static int nt_cluster(const NsArgs& q) {
   const int narrow = std::min(kNtMaxCluster, (q.large + 127) / 128), wide = (q.large + kNtMaxCols - 1) / kNtMaxCols;
   return wide > 1 && tiles * narrow <= sm_count() * 4 / 5 ? narrow : wide;
 }
-// whether there are more tiles than clusters on the GPU
-static bool ns_many(const NsArgs& q) {
-  const int64_t pack = kNtRows / q.small;
-  return (q.count + pack - 1) / pack * ((q.large + kNtMaxCols - 1) / kNtMaxCols) > sm_count();
+// the kernel for `count` matrices (the rule: at kNsWarpFew)
+enum NsKernel { kNsWarp, kNsPair, kNsCluster };
+static NsKernel ns_kernel(int64_t count, int small, int large) {
+  const int64_t pack = kNtRows / small;
+  // more tiles than clusters on the GPU
+  const bool many = (count + pack - 1) / pack * ((large + kNtMaxCols - 1) / kNtMaxCols) > sm_count();
+  if (small <= kNsWarpRows) return large <= kNsWarpFew || (large <= kNsWarpLong[small > 16] && many) ? kNsWarp : kNsCluster;
+  if (small <= kNsPairRows) return large <= kNsPairFew || (large <= kNsPairLong && many) ? kNsPair : kNsCluster;
+  return kNsCluster;
+}
+// whether the kernel is the one with bounded waits
+static bool ns_waits(int64_t count, int rows, int cols) {
+  return count > 0 && ns_kernel(count, std::min(rows, cols), std::max(rows, cols)) == kNsCluster;
 }
 
 int launch_ns_cluster(const NsArgs& q, cudaStream_t st, bool launch) {
@@ -546,12 +555,8 @@ static int ns_launch(const char* who, NsArgs& q, int64_t n, int32_t rows, int32_
   if (!tall)
     for (int v = 2; v <= 4; v *= 2)
       if (cols % v == 0 && wide % (4 * v) == 0 && typed % (size * v) == 0) q.vec = v;
-  if (q.small <= kNsWarpRows) {
-    if (q.large <= kNsWarpFew || (q.large <= kNsWarpLong[q.small > 16] && ns_many(q))) return launch_ns_warp(q, st, stage == kNsLaunch);
-  } else if (q.small <= kNsPairRows) {
-    if (q.large <= kNsPairFew || (q.large <= kNsPairLong && ns_many(q))) return launch_ns_pair(q, st, stage == kNsLaunch);
-  }
-  return launch_ns_cluster(q, st, stage == kNsLaunch);
+  const NsKernel kernel = ns_kernel(q.count, q.small, q.large);
+  return (kernel == kNsWarp ? launch_ns_warp : kernel == kNsPair ? launch_ns_pair : launch_ns_cluster)(q, st, stage == kNsLaunch);
 }
 
 }  // namespace mlpsp
@@ -561,22 +566,25 @@ using namespace mlpsp;
 namespace mlpsp {
 static thread_local int32_t g_withhold = 0;
 
-// the answer of a call's waits, for which the call waits
+// the answer of a call's waits, for which the call waits, if it has any
 struct NsAnswer {
   int32_t* to;
   HostWords& hw;
   cudaEvent_t ev = nullptr;
   explicit NsAnswer(int32_t* host) : to(host), hw(host_words()) {}
-  int open(NsArgs& q) {
+  int open(NsArgs& q, bool waits) {
     if (!to) return MLPSP_OK;
+    *to = 0;
+    if (!waits) return MLPSP_OK;
     const int rc = hw.open(&ev);
     if (rc) return rc;
     hw.word[0] = 0;
     q.gave_up = static_cast<volatile int32_t*>(hw.word);
     return MLPSP_OK;
   }
+  // also behind a launch that failed: the kernels before it still write the word
   int read(cudaStream_t st) {
-    if (!to) return MLPSP_OK;
+    if (!ev) return MLPSP_OK;
     MLPSP_CUDA_OK(cudaEventRecord(ev, st));
     MLPSP_CUDA_OK(cudaEventSynchronize(ev));
     *to = *static_cast<volatile int32_t*>(hw.word);
@@ -596,6 +604,11 @@ extern "C" int mlpsp_orthogonalize_waits(int32_t rows, int32_t cols) {
   return small > kNsPairRows || large > (small <= kNsWarpRows ? kNsWarpFew : kNsPairFew) ? 1 : 0;
 }
 
+extern "C" int mlpsp_orthogonalize_stack_waits(int64_t n, int32_t rows, int32_t cols) {
+  const bool sizes = rows >= 1 && cols >= 1 && std::min(rows, cols) <= MLPSP_MUON_MAX_SMALL && std::max(rows, cols) <= MLPSP_MUON_MAX_LARGE;
+  return sizes && ns_waits(n, rows, cols) ? 1 : 0;
+}
+
 extern "C" int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n, int32_t rows, int32_t cols, int32_t steps, double a,
                                    double b, double c, double eps, void* out, int32_t* gave_up_host, void* stream) {
   NsArgs q = {};
@@ -605,7 +618,7 @@ extern "C" int mlpsp_orthogonalize(const void* update, int32_t dtype, int64_t n,
   q.withhold = g_withhold;
   NsAnswer answer(gave_up_host);
   int rc = ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream, kNsCheck);
-  if (!rc) rc = answer.open(q);
+  if (!rc) rc = answer.open(q, ns_waits(n, rows, cols));
   if (!rc) rc = ns_launch("mlpsp_orthogonalize", q, n, rows, cols, steps, a, b, c, eps, (cudaStream_t)stream, kNsLaunch);
   return rc ? rc : answer.read((cudaStream_t)stream);
 }
@@ -619,11 +632,12 @@ extern "C" int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, 
                 "mlpsp_muon_step: lr and weight_decay must be finite and not negative");
   NsAnswer answer(gave_up_host);
   // all tensors are checked, and their kernels allowed the shared memory that they take, before the first launch
+  bool waits = false;
   for (const NsStage stage : {kNsCheck, kNsPrepare, kNsLaunch}) {
     bool follows = false;
     NsArgs shared = {};
     if (stage == kNsLaunch) {
-      const int rc = answer.open(shared);
+      const int rc = answer.open(shared, waits);
       if (rc) return rc;
     }
     for (int32_t i = 0; i < count; ++i) {
@@ -645,7 +659,11 @@ extern "C" int mlpsp_muon_step(const mlpsp_muon_tensor* tensors, int32_t count, 
       q.step = (float)(lr * t.scale);
       q.follows = follows;
       const int rc = ns_launch("mlpsp_muon_step", q, t.n, t.rows, t.cols, steps, a, b, c, eps, (cudaStream_t)stream, stage);
-      if (rc) return rc;
+      if (rc) {
+        if (follows) answer.read((cudaStream_t)stream);
+        return rc;
+      }
+      waits |= ns_waits(t.n, t.rows, t.cols);
       follows |= t.n > 0;
     }
   }

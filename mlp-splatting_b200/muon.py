@@ -41,10 +41,10 @@ def _check_tensors(tensors):
 
 def _answer(shapes, check):
     """A word for the answer of kernels that wait on the device, or None."""
-    if not check or not any(L.load().mlpsp_orthogonalize_waits(rows, cols) for _n, rows, cols in shapes):
+    if not check or not any(L.load().mlpsp_orthogonalize_stack_waits(*shape) for shape in shapes):
         return None
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("matrices of these sizes wait for the kernel's answer: pass check=False inside a graph capture")
+        raise RuntimeError("matrices of these sizes and this number wait for the kernel's answer: pass check=False inside a graph capture")
     return C.c_int32(0)
 
 

@@ -61,3 +61,10 @@ def test_routes_off_their_elements():
         return L.load().mlpsp_route_records(ids, 4, 600, first, 2, offsets, slots, scratch, 1 << 20, None, None)
 
     misaligned(route, ids=4, first=8, offsets=8, slots=4, scratch=4)
+
+
+def test_which_stacks_wait():
+    """The cluster kernel's: by size, or by size and number (of 148 SMs, where no device answers)."""
+    waits = L.load().mlpsp_orthogonalize_stack_waits
+    assert [waits(*s) for s in ((1, 32, 800), (4000, 32, 800), (4000, 32, 801), (1, 64, 384), (4000, 64, 384), (4000, 384, 65))] == [1, 0, 1, 1, 0, 1]
+    assert [waits(*s) for s in ((0, 128, 128), (-1, 128, 128), (1, 0, 4), (1, 129, 129), (1, 4, 2049), (1, 32, 512), (1, 256, 64))] == [0] * 7

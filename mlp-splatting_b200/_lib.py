@@ -22,6 +22,7 @@ BIT_PIXEL_HITS = 32
 ORDER_PER_PIXEL = 2
 REVERSE_BAD_OFFSETS, REVERSE_BAD_IDS = 1, 2
 ROUTE_BAD_OFFSETS, ROUTE_MAX_DIM = 1, 65536
+E_CUDA = -3      # a CUDA call failed, which launches before it may not have
 MUON_MAX_SMALL, MUON_MAX_LARGE = 128, 2048
 PRECISION_F32, PRECISION_F16, PRECISION_BF16 = 0, 1, 2
 MAX_WAVES = 32

@@ -53,9 +53,12 @@ def _read(answer, what):
         raise RuntimeError(f"{what}: a device-side wait gave up; results are invalid")
 
 
-def _written(tensors):
-    """In-place writes count as such: scenes packed from the old weights are packed anew, autograd sees saved tensors change."""
-    increment_version([t for t in tensors if not t.is_inference()])
+def _written(rc, what, tensors):
+    """In-place writes count as such: scenes packed from the old weights are packed anew, autograd sees saved tensors change.  Also those of the
+    launches before one that failed, if the library's call did (rc)."""
+    if rc in (0, L.E_CUDA):
+        increment_version([t for t in tensors if not t.is_inference()])
+    L.check(rc, what)
 
 
 def _coefficients(coefficients, steps, eps):
@@ -93,9 +96,9 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     dev = _check_tensors([update, out])
     with _on(dev):
         answer = _answer([(n, rows, cols)], check)
-        L.check(L.load().mlpsp_orthogonalize(L.ptr(update), _TYPES[update.dtype], n, rows, cols, *args, L.ptr(out),
-                                             None if answer is None else C.byref(answer), _stream_ptr(dev)), "mlpsp_orthogonalize")
-    _written([out])
+        rc = L.load().mlpsp_orthogonalize(L.ptr(update), _TYPES[update.dtype], n, rows, cols, *args, L.ptr(out),
+                                          None if answer is None else C.byref(answer), _stream_ptr(dev))
+    _written(rc, "mlpsp_orthogonalize", [out])
     _read(answer, "orthogonalize")
     return out
 
@@ -147,7 +150,7 @@ def muon_step(weights, grads, momenta, *, lr: float, momentum: float = 0.95, nes
         tensors = (L.MuonTensor * len(shapes))(*(
             (L.ptr(w), L.ptr(g), L.ptr(m), n, rows, cols, math.sqrt(max(1.0, rows / cols)), _TYPES[g.dtype], 0)
             for w, g, m, (n, rows, cols) in zip(*lists, shapes)))
-        L.check(lib.mlpsp_muon_step(tensors, len(shapes), L.ptr(active), lr, momentum, int(bool(nesterov)), weight_decay, *args,
-                                    None if answer is None else C.byref(answer), _stream_ptr(dev)), "mlpsp_muon_step")
-    _written(lists[0] + lists[2])
+        rc = lib.mlpsp_muon_step(tensors, len(shapes), L.ptr(active), lr, momentum, int(bool(nesterov)), weight_decay, *args,
+                                 None if answer is None else C.byref(answer), _stream_ptr(dev))
+    _written(rc, "mlpsp_muon_step", lists[0] + lists[2])
     _read(answer, "muon_step")

@@ -239,16 +239,19 @@ def _combine(y, route, weights, name="y"):
     return out
 
 
-def _combine_gradients(grad_out, y, route, weights, want_y, want_weights):
+def _combine_gradients(grad_out, y, route, weights, want_y, weights_shape):
+    """y may be None without weights_shape (the gradient of y does not read it), weights None for ones or without want_y."""
     dev = _check_route(route, grad_out, y, weights)
     _check_rows("grad_out", grad_out, route.pixels)
-    _check_rows("y", y, route.slots.numel())
-    if y.dtype != grad_out.dtype or y.shape[1] != grad_out.shape[1]:
-        raise ValueError("grad_out and y must have one element type and row length")
-    grad_y = torch.empty_like(y) if want_y else None
-    grad_weights = torch.empty_like(weights) if want_weights else None
-    if want_y or want_weights:
-        _call("mlpsp_combine_rows_gradients", dev, grad_out.data_ptr(), y.data_ptr(), _ROW_TYPES[y.dtype], y.shape[1], L.ptr(weights),
+    if y is not None:
+        _check_rows("y", y, route.slots.numel())
+        if y.dtype != grad_out.dtype or y.shape[1] != grad_out.shape[1]:
+            raise ValueError("grad_out and y must have one element type and row length")
+    dim = grad_out.shape[1]
+    grad_y = grad_out.new_empty((route.slots.numel(), dim)) if want_y else None
+    grad_weights = None if weights_shape is None else grad_out.new_empty(weights_shape, dtype=torch.float32)
+    if want_y or weights_shape is not None:
+        _call("mlpsp_combine_rows_gradients", dev, grad_out.data_ptr(), L.ptr(y), _ROW_TYPES[grad_out.dtype], dim, L.ptr(weights),
               *_route_args(route), L.ptr(grad_y), L.ptr(grad_weights))
     return grad_y, grad_weights
 
@@ -273,7 +276,9 @@ class _DispatchRows(torch.autograd.Function):
 class _CombineRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, route, weights):
-        ctx.save_for_backward(y, weights, route.offsets, route.slots, route.pixel_offsets)
+        ctx.weights_shape = weights.shape if weights is not None and ctx.needs_input_grad[2] else None
+        ctx.save_for_backward(None if ctx.weights_shape is None else y, weights if ctx.needs_input_grad[0] else None, route.offsets, route.slots,
+                              route.pixel_offsets)
         ctx.pixels, ctx.fan = route.pixels, route.fan
         return _combine(y, route, weights)
 
@@ -282,7 +287,7 @@ class _CombineRows(torch.autograd.Function):
     def backward(ctx, grad):
         y, weights, *where = ctx.saved_tensors
         grad_y, grad_weights = _combine_gradients(grad.contiguous(), y, _saved_route(ctx, *where), weights, ctx.needs_input_grad[0],
-                                                  weights is not None and ctx.needs_input_grad[2])
+                                                  ctx.weights_shape if ctx.needs_input_grad[2] else None)
         return grad_y, None, grad_weights
 
 
@@ -321,4 +326,4 @@ def combine_rows_gradients(grad_out: torch.Tensor, y: torch.Tensor, route: Recor
     """(gradient of combine_rows with respect to y [records, D], with respect to weights in their shape, or None without
     weights) from grad_out [pixels, D].  Zero for dropped records."""
     _refuse_tangents("combine_rows_gradients", (grad_out, y, weights))
-    return _combine_gradients(grad_out, y, route, weights, True, weights is not None)
+    return _combine_gradients(grad_out, y, route, weights, True, None if weights is None else weights.shape)

@@ -6,8 +6,8 @@
 // eleven bits would put errors of tenths into an orthogonal matrix.  X, A and bA + cA^2 are held as binary16 pairs hi + lo
 // (22 bits; X and A, whose entries become small, scaled by 2^10, so that their absolute error stays below 3e-11), every product is
 // hi hi + hi lo + lo hi on the tensor cores with FP32 accumulation, and a X is added in FP32, with the diagonals of A, A^2 and P.  On
-// Gaussian matrices the result is then nearer to 64-bit arithmetic than an iteration in plain FP32: 8e-7 and 9.5e-7 (32 x 72), 7e-7 and
-// 1e-6 (64 x 72), 1.1e-6 and 2.5e-6 (128 x 1152).
+// Gaussian matrices the result is then nearer to 64-bit arithmetic than an iteration in plain FP32: 8.5e-7 and 1.2e-6 (32 x 72), 8.0e-7 and
+// 1.2e-6 (64 x 72), 6.6e-7 and 2.0e-6 (128 x 1152).
 #pragma once
 #include <type_traits>
 #include "frame.cuh"

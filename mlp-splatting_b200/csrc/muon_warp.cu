@@ -317,8 +317,8 @@ __global__ void __launch_bounds__(32, CTAS) k_ns_warp(const NsArgs q, const int 
 #pragma unroll 1
         for (int p = 0; p < kWhole; ++p) columns(p, NsTag<2>{});
       } else {
-        // Long rows, four panels at a time, whose sums are added in FP32: the tensor core rounds towards zero with every MMA, and over 1,500
-        // columns that came to 6e-6 of the result
+        // Long rows, four panels at a time, whose sums are added in FP32: the tensor core rounds towards zero with every MMA, which came to
+        // 6.4e-6 of the result for 16 x 1024 and 6.6e-6 for 32 x 800, so to 4.7e-7 and 9.5e-7
         float sum[MB * (MB + 1)][4];
 #pragma unroll
         for (int i = 0; i < MB * (MB + 1); ++i) sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.f;

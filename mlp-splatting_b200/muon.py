@@ -1,7 +1,8 @@
 """Weight updates by orthogonalised momentum, for the primitives' layers and the feature decoder's.
 
 The step that follows primitive_gemm.grouped_weight_gradients: the gradient's running mean is taken to the nearest matrix with
-singular values of about one by a Newton-Schulz iteration, matrix by matrix, and subtracted from the weights.  Works on stacks of
+singular values of about one by a Newton-Schulz iteration, matrix by matrix, and subtracted from the weights.  The rule and its coefficients are
+those of K. Jordan and others, "Muon: An optimizer for hidden layers in neural networks" (2024).  Works on stacks of
 matrices ([N, 32, 72], [N, 32, 32] and [N, 4, 32] of a scene) and on single ones; biases and other vectors are left to the caller's
 own rule.  There is no CPU path.
 """

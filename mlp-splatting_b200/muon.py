@@ -80,9 +80,11 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, coefficients=COEFFICI
     update: float32, float16 or bfloat16, [rows, columns] or [N, rows, columns], contiguous; out (update itself, or a tensor
     apart from it) receives the result in update's type.  The iteration has FP32 accuracy whatever the type.  A matrix of zeros stays
     zero; one that holds an infinity or a NaN becomes NaN and touches no other.  Coefficients under which singular values leave
-    [0, 4] are refused.  There is no gradient: the result does not require grad, and inputs with forward-mode tangents are refused.  Large matrices (more than 64 rows on the shorter side, or more than 512, with 33 to 64 rows 256, on the
-    longer) may go to a kernel with bounded waits, for whose answer the call waits (RuntimeError if one gave up) unless check is False, where
-    only NaN in the result shows it; their number decides on the kernel and on the CTAs that share a matrix, which shows in the last bits."""
+    [0, 4] are refused.  There is no gradient: the result does not require grad, and inputs with forward-mode tangents are refused.
+
+    Large matrices (more than 64 rows on the shorter side, or more than 512, with 33 to 64 rows 256, on the longer) may go to a kernel
+    with bounded waits, for whose answer the call waits (RuntimeError if one gave up) unless check is False, where only NaN in the
+    result shows it; their number decides on the kernel and on the CTAs that share a matrix, which shows in the last bits."""
     _refuse_tangents("orthogonalize", (update, out))
     n, rows, cols = _shape("update", update)
     if update.dtype not in _TYPES:

@@ -208,8 +208,10 @@ def route_records(primitive_ids: torch.Tensor, num_primitives: int, pixel_offset
         primitive_ids = primitive_ids.clamp(-1, n).to(torch.int32)
     lib, dev = L.load(), primitive_ids.device
     ids = primitive_ids.contiguous()
-    if first is not None and check and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("route_records waits for the check of pixel_offsets: pass check=False inside a graph capture")
+    if first is not None and check:
+        with _on(dev):      # the stream that the call is for
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("route_records waits for the check of pixel_offsets: pass check=False inside a graph capture")
     offsets = torch.empty(n + 1, device=dev, dtype=torch.int64)
     slots = torch.empty(R, device=dev, dtype=torch.int32)
     nbytes = int(lib.mlpsp_route_records_scratch_bytes(R, n))

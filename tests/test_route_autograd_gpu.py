@@ -75,3 +75,25 @@ def test_backward_in_a_graph():
         torch.cuda.synchronize()
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+def test_the_capture_that_counts_is_that_of_the_ids_device(monkeypatch):
+    """With ids on another device than the current one it is that device's stream that may be capturing."""
+    entered, asked, real = [], [], torch.cuda.is_current_stream_capturing
+
+    class On(pc._on):
+        __slots__ = ()
+
+        def __enter__(self):
+            entered.append(self.d)
+            return super().__enter__()
+
+        def __exit__(self, *exc):
+            entered.pop()
+            return super().__exit__(*exc)
+
+    monkeypatch.setattr(pc, "_on", On)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: (asked.append(list(entered)), real())[1])
+    ids = torch.zeros(6, dtype=torch.int32, device="cuda")
+    pc.route_records(ids, 2, torch.tensor([0, 2, 6], device="cuda"))
+    assert asked == [[ids.device]]
